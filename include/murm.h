@@ -366,6 +366,54 @@ MURM_API murm_status murm_decode_step(const murm_decode_args* args, void* stream
 MURM_API murm_status murm_phase_sizes(const murm_phase_shape* shape, size_t* update_saved_bytes,
                                       size_t* workspace_bytes);
 
+/* Per-head RMS norm with the position rotation in the same pass, and the
+ * rotation alone (no counterpart in the reference, whose q goes from the
+ * projection to the select as it is). For every row x [head_dim] of q and k:
+ *
+ *   u = x * rsqrt(mean(x^2) + eps) * weight     (normalize; else u = x)
+ *   y = u with each of its rotary_dim / 2 pairs turned by the angle
+ *       position[axis of the pair] * frequency of the pair
+ *
+ * Pair i is (u[i], u[i + rotary_dim/2]), or (u[2i], u[2i+1]) when interleaved;
+ * elements from rotary_dim on pass through. `axes` positions per token
+ * (1 to 4); sections[a] pairs, in order, turn by axis a (axes = 1 needs no
+ * sections). Frequencies: base^(-2i/rotary_dim) for pair i of the head, or,
+ * with own_spectrum, base^(-j/sections[a]) for the j-th pair of axis a, or
+ * the caller's freqs[i]. Angles are formed in 64 bits and reduced to one turn
+ * before the 32-bit sine and cosine, so long contexts lose no accuracy.
+ *
+ * The backward takes the same arguments with `grad` set and writes dL/dx to
+ * `out` and, where grad_weight is not NULL, dL/dweight (in the weight's type;
+ * needs the workspace). Without normalize the backward is the forward with
+ * `inverse` set (the transposed rotation) applied to the gradient. */
+typedef enum murm_position_type { MURM_POS_I64 = 0, MURM_POS_I32 = 1, MURM_POS_F32 = 2 } murm_position_type;
+
+typedef struct murm_head_rows {               /* one tensor [B, heads, N, head_dim] */
+  const void* x; int64_t x_stride[3];         /* {batch, head, token}, unit inner stride */
+  const void* grad; int64_t grad_stride[3];   /* backward: dL/dy */
+  void* out; int64_t out_stride[3];           /* y, or dL/dx in the backward */
+  const void* weight;                         /* [head_dim], or NULL (all ones) */
+  void* grad_weight;                          /* backward: [head_dim], or NULL */
+  int32_t heads;                              /* 0: the tensor is absent */
+  int32_t weight_dtype;                       /* murm_dtype of weight and grad_weight: MURM_F32 or `dtype` */
+} murm_head_rows;
+
+typedef struct murm_norm_rope_args {
+  int32_t batch, tokens, head_dim, rotary_dim; /* head_dim even, 2..256; rotary_dim even, 0..head_dim */
+  int32_t dtype, normalize, interleaved, inverse;
+  int32_t axes, sections[4], own_spectrum;
+  int32_t position_type;                       /* murm_position_type */
+  double eps, base;
+  const void* positions; int64_t position_stride[3]; /* {batch, token, axis}; 0 broadcasts */
+  const float* freqs;                          /* [rotary_dim / 2], or NULL */
+  murm_head_rows q, k;
+  void* workspace; size_t workspace_bytes;     /* backward with a grad_weight */
+} murm_norm_rope_args;
+MURM_API murm_status murm_norm_rope_fwd(const murm_norm_rope_args* args, void* stream);
+MURM_API murm_status murm_norm_rope_bwd(const murm_norm_rope_args* args, void* stream);
+/* Bytes of the backward's workspace (whatever the sizes and types). */
+MURM_API size_t murm_norm_rope_workspace(void);
+
 /* Launch accounting and per-kernel timing (host-side instrumentation; no
  * effect on results). murm_kernel_launches() counts every kernel this library
  * has launched in the process. Between murm_profile_begin() and

@@ -202,6 +202,34 @@ class HostStepArgs(ctypes.Structure):
     ]
 
 
+MURM_POS_I64, MURM_POS_I32, MURM_POS_F32 = 0, 1, 2
+
+
+class HeadRows(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_stride", Strides),
+        ("grad", ctypes.c_void_p), ("grad_stride", Strides),
+        ("out", ctypes.c_void_p), ("out_stride", Strides),
+        ("weight", ctypes.c_void_p), ("grad_weight", ctypes.c_void_p),
+        ("heads", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+    ]
+
+
+class NormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("normalize", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4), ("own_spectrum", ctypes.c_int32),
+        ("position_type", ctypes.c_int32),
+        ("eps", ctypes.c_double), ("base", ctypes.c_double),
+        ("positions", ctypes.c_void_p), ("position_stride", Strides),
+        ("freqs", ctypes.c_void_p),
+        ("q", HeadRows), ("k", HeadRows),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # Every symbol include/murm.h declares; tests check the library exports them all.
 EXPORTS = (
     "murm_slot_murmurate_sizes",
@@ -229,6 +257,9 @@ EXPORTS = (
     "murm_slot_sums_bwd",
     "murm_host_step_sizes",
     "murm_slot_murmurate_host_step",
+    "murm_norm_rope_fwd",
+    "murm_norm_rope_bwd",
+    "murm_norm_rope_workspace",
 )
 
 STATUS_NAMES = {
@@ -286,10 +317,13 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                          ("murm_slot_update_fwd", SlotUpdateArgs), ("murm_slot_update_bwd", SlotUpdateBwdArgs),
                          ("murm_slot_diffusion_fwd", SlotDiffusionArgs),
                          ("murm_slot_diffusion_bwd", SlotDiffusionArgs), ("murm_decode_step", DecodeArgs),
-                         ("murm_slot_sums_fwd", SlotSumsArgs), ("murm_slot_sums_bwd", SlotSumsBwdArgs)):
+                         ("murm_slot_sums_fwd", SlotSumsArgs), ("murm_slot_sums_bwd", SlotSumsBwdArgs),
+                         ("murm_norm_rope_fwd", NormRopeArgs), ("murm_norm_rope_bwd", NormRopeArgs)):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
             fn.restype = ctypes.c_int
+        lib.murm_norm_rope_workspace.argtypes = []
+        lib.murm_norm_rope_workspace.restype = ctypes.c_size_t
         lib.murm_host_step_sizes.argtypes = [ctypes.POINTER(Shape), ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]
         lib.murm_host_step_sizes.restype = ctypes.c_int
         lib.murm_slot_murmurate_host_step.argtypes = [ctypes.POINTER(HostStepArgs), ctypes.c_void_p]
