@@ -414,6 +414,60 @@ MURM_API murm_status murm_norm_rope_bwd(const murm_norm_rope_args* args, void* s
 /* Bytes of the backward's workspace (whatever the sizes and types). */
 MURM_API size_t murm_norm_rope_workspace(void);
 
+/* Linear layer with its bias, activation and residual in one call (no
+ * counterpart in the reference, whose projections are torch modules around the
+ * op, README.md:82-102):
+ *
+ *   z = x W^T + bias,  out = act(z) + residual
+ *
+ * x [rows, in_features] and weight [out_features, in_features] of `dtype`
+ * with unit inner stride and the given row strides (any element alignment),
+ * residual and out [rows, out_features] likewise, bias [out_features]. Sums
+ * are in fp32 (fp32 inputs: exact three-term bf16 splits, fp32 accuracy).
+ * preact, when not NULL, receives z in `dtype` ([rows, out_features]
+ * contiguous) for the backward; it is needed there unless the activation is
+ * MURM_ACT_NONE.
+ *
+ * Backward: dz = grad_out * act'(z), rounded once to `dtype` where it becomes a
+ * matrix operand; grad_x = dz W, grad_weight = dz^T x, grad_bias = column sums of
+ * the unrounded dz (fixed order). Each output may be NULL. rows may be 0. */
+typedef enum murm_activation {
+  MURM_ACT_NONE = 0, MURM_ACT_RELU = 1, MURM_ACT_SILU = 2,
+  MURM_ACT_GELU = 3,      /* z Phi(z), with the error function */
+  MURM_ACT_GELU_TANH = 4  /* its tanh form */
+} murm_activation;
+
+typedef struct murm_linear_args {
+  int64_t rows;
+  int32_t in_features, out_features, dtype, activation;
+  const void* x; int64_t x_stride;
+  const void* weight; int64_t w_stride;
+  const void* bias;                           /* or NULL */
+  const void* residual; int64_t r_stride;     /* or NULL */
+  void* out; int64_t out_stride;
+  void* preact;                               /* or NULL */
+  void* workspace; size_t workspace_bytes;
+} murm_linear_args;
+
+typedef struct murm_linear_bwd_args {
+  int64_t rows;
+  int32_t in_features, out_features, dtype, activation;
+  const void* x; int64_t x_stride;
+  const void* weight; int64_t w_stride;
+  const void* preact;                         /* as the forward wrote it */
+  const void* grad_out; int64_t go_stride;
+  void* grad_x; int64_t gx_stride;            /* each gradient: or NULL */
+  void* grad_weight; int64_t gw_stride;
+  void* grad_bias;
+  void* workspace; size_t workspace_bytes;
+} murm_linear_bwd_args;
+
+MURM_API murm_status murm_linear_fwd(const murm_linear_args* args, void* stream);
+MURM_API murm_status murm_linear_bwd(const murm_linear_bwd_args* args, void* stream);
+/* Workspace bytes of a call with these arguments (its workspace fields are not read). */
+MURM_API murm_status murm_linear_workspace(const murm_linear_args* args, size_t* bytes);
+MURM_API murm_status murm_linear_bwd_workspace(const murm_linear_bwd_args* args, size_t* bytes);
+
 /* Launch accounting and per-kernel timing (host-side instrumentation; no
  * effect on results). murm_kernel_launches() counts every kernel this library
  * has launched in the process. Between murm_profile_begin() and

@@ -230,6 +230,35 @@ class NormRopeArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("w_stride", ctypes.c_int64),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p), ("r_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+        ("preact", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("w_stride", ctypes.c_int64),
+        ("preact", ctypes.c_void_p),
+        ("grad_out", ctypes.c_void_p), ("go_stride", ctypes.c_int64),
+        ("grad_x", ctypes.c_void_p), ("gx_stride", ctypes.c_int64),
+        ("grad_weight", ctypes.c_void_p), ("gw_stride", ctypes.c_int64),
+        ("grad_bias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # Every symbol include/murm.h declares; tests check the library exports them all.
 EXPORTS = (
     "murm_slot_murmurate_sizes",
@@ -260,6 +289,10 @@ EXPORTS = (
     "murm_norm_rope_fwd",
     "murm_norm_rope_bwd",
     "murm_norm_rope_workspace",
+    "murm_linear_fwd",
+    "murm_linear_bwd",
+    "murm_linear_workspace",
+    "murm_linear_bwd_workspace",
 )
 
 STATUS_NAMES = {
@@ -318,10 +351,14 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                          ("murm_slot_diffusion_fwd", SlotDiffusionArgs),
                          ("murm_slot_diffusion_bwd", SlotDiffusionArgs), ("murm_decode_step", DecodeArgs),
                          ("murm_slot_sums_fwd", SlotSumsArgs), ("murm_slot_sums_bwd", SlotSumsBwdArgs),
-                         ("murm_norm_rope_fwd", NormRopeArgs), ("murm_norm_rope_bwd", NormRopeArgs)):
+                         ("murm_norm_rope_fwd", NormRopeArgs), ("murm_norm_rope_bwd", NormRopeArgs),
+                         ("murm_linear_fwd", LinearArgs), ("murm_linear_bwd", LinearBwdArgs)):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
             fn.restype = ctypes.c_int
+        for name, st in (("murm_linear_workspace", LinearArgs), ("murm_linear_bwd_workspace", LinearBwdArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(st), ctypes.POINTER(ctypes.c_size_t)]
+            getattr(lib, name).restype = ctypes.c_int
         lib.murm_norm_rope_workspace.argtypes = []
         lib.murm_norm_rope_workspace.restype = ctypes.c_size_t
         lib.murm_host_step_sizes.argtypes = [ctypes.POINTER(Shape), ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]
