@@ -220,7 +220,7 @@ murm_status murm_device_status(void* stream) {
   if (e != cudaSuccess) return cuda_status(e, "murm_device_status");
   if (code)
     return fail(MURM_ERR_DEVICE, "a kernel gave up waiting (error bits 0x%x: 1 operand copy, 2 token tile copy, "
-                "4 tensor-core completion, 8 backward copy or MMA, 16 wait probe, 32 another CTA's round)", code);
+                "4 tensor-core completion, 8 backward copy or MMA, 16 wait probe, 32 another CTA's round, 64 linear copy or MMA)", code);
   return MURM_OK;
 }
 

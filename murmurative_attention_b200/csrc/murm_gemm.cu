@@ -1,56 +1,761 @@
-// murm_gemm.cu — matrix product with the linear layer's epilogue.
+// murm_gemm.cu — the linear layer's matrix products on tcgen05, with their epilogue.
+//
+// D = A B^T with A [M][K], B [N][K] read as they lie in memory: the tensor cores take either
+// operand K-major (rows of K) or MN-major (rows of M or N), so the forward (x W^T) and both
+// gradients (dz W, dz^T x) need no transposed copy.
+//
+// k_gemm_tc: a pair of CTAs (cta_group::2) per 256 x BN tile, each holding 128 rows of A, half the
+// rows of B and a 128 x BN fp32 accumulator in TMEM (two accumulators: a tile's epilogue runs under
+// the next tile's products). Persistent over the tiles. Warp 0 loads the operands by TMA into a
+// ring of 64-deep stages, warp 1 of the first CTA issues the MMAs of both, warp 3 loads residual
+// tiles, warps 4-7 run the epilogue: TMEM -> registers -> bias, activation, residual -> 128-byte
+// swizzled rows in shared memory -> TMA store (or plain stores where the result's rows are not
+// 16-byte aligned).
+//
+// fp32 operands are three bf16 planes; the products of planes (i, j) with i + j <= 2 carry them to
+// 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K
+// split K; the parts' fp32 sums go to the workspace and k_split_sum adds them in order and runs the
+// epilogue.
+#include <cudaTypedefs.h>
+
+#include <cstdio>
+
 #include "murm_linear.cuh"
+#include "murm_sm100.cuh"
 
 namespace murm {
-namespace lin {
 
-// 64 x 64 tile per block, 4 x 4 outputs per thread, products and sums in fp32.
+extern __device__ int g_device_error;
+PFN_cuTensorMapEncodeTiled_v12000 tc_tensor_map_encoder();  // murm_tc.cu
+
+namespace lin {
+using namespace sm100;
+
+constexpr int kErrLinear = 64;  // device error bit: a copy or an MMA of a linear product never completed
+constexpr int kSms = 148;
+constexpr int kPairs = kSms / 2;     // CTA pairs resident at once
+constexpr int kBK = 64;              // depth of a stage: one 128-byte swizzled row
+constexpr uint32_t kABytes = 128 * kBK * 2;
+constexpr int kEpiWarps = 4;
+constexpr int kThreads = 256;
+constexpr uint32_t kBuf = 32 * 128;  // one epilogue warp's 32 rows of 128 bytes
+
+template <int BN> struct Tile {
+  static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
+  static constexpr uint32_t kStage = kABytes + kBBytes;
+  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr uint32_t OFF_OUT = kStages * kStage;            // [warp][2] result buffers
+  static constexpr uint32_t OFF_RES = OFF_OUT + kEpiWarps * 2 * kBuf;  // [warp][2] residual buffers
+  static constexpr uint32_t OFF_BIAS = OFF_RES + kEpiWarps * 2 * kBuf;
+  static constexpr uint32_t OFF_BAR = OFF_BIAS + kEpiWarps * 64 * 4;
+  static constexpr uint32_t kSmem = OFF_BAR + 512 + 1024;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static_assert(kSmem <= 232448, "shared memory budget");
+};
+
+struct Bars {  // in shared memory at OFF_BAR
+  uint64_t full[8], empty[8];        // operand stages; `full` of the pair's first CTA counts both loads
+  uint64_t acc_full[2], acc_free[2];  // accumulators; acc_free is used in the pair's first CTA
+  uint64_t res_full[kEpiWarps][2], res_free[kEpiWarps][2];
+  uint32_t tmem;
+};
+static_assert(sizeof(Bars) <= 512, "barrier area");
+
+struct Args {
+  int M, N;
+  int kblocks, iters, total, splits;  // stages per plane pair, per split, in all; K splits
+  int tiles_n, tiles, items;          // items: tiles * splits
+  uint32_t idesc;
+  int a_mn, b_mn;
+  int fp32;  // operands are three planes
+  const void* bias;
+  int act;
+  const void* res; int64_t ldr; int res_tma;
+  void* out; int64_t ldo; int out_tma;
+  void* pre; int pre_tma;
+  int split_rows;  // rows of one split's partial result
+};
+
+// Plane pairs of an fp32 product, smallest terms first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0).
+__device__ __forceinline__ int plane_a(int pair) { return (0x021010 >> (4 * (5 - pair))) & 15; }
+__device__ __forceinline__ int plane_b(int pair) { return (0x201100 >> (4 * (5 - pair))) & 15; }
+
+// ---------------------------------------------------------------------------
+// PTX of the CTA pair
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+// The address of the first CTA's copy of a shared-memory object.
+__device__ __forceinline__ uint32_t map_to_first(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Load into this CTA's shared memory that counts on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                              uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
+      "%3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// All but the newest N of this thread's stores have read their shared memory.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once this thread's MMAs are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  if (mbar_timed_wait(bar, parity)) return true;
+  atomicOr(&g_device_error, kErrLinear);
+  return false;
+}
+
+// ---------------------------------------------------------------------------
+// epilogue pieces
+// ---------------------------------------------------------------------------
+template <typename T> struct Out {  // 16-bit results: 64 columns in a 128-byte row
+  static constexpr int kCols = 64;
+  static constexpr bool kFast = true;
+};
+template <> struct Out<float> {
+  static constexpr int kCols = 32;
+  static constexpr bool kFast = false;
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t u, const __half*) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t u, const __nv_bfloat16*) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A lane's 128-byte row of a swizzled buffer: chunk j of 16 bytes sits at j ^ (row mod 8).
 template <typename T>
-__global__ void __launch_bounds__(256) k_gemm(Gemm g) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const T* a = static_cast<const T*>(g.a);
-  const T* b = static_cast<const T*>(g.b);
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < g.K; k0 += 16) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int ka = g.a_mn ? i >> 6 : i & 15, ma = g.a_mn ? i & 63 : i >> 4;
-      const int kb = g.b_mn ? i >> 6 : i & 15, nb = g.b_mn ? i & 63 : i >> 4;
-      const int64_t m = m0 + ma, n = n0 + nb, k1 = k0 + ka, k2 = k0 + kb;
-      sa[ka][ma] = m < g.M && k1 < g.K ? Elem<T>::load(a + (g.a_mn ? k1 * g.lda + m : m * g.lda + k1)) : 0.f;
-      sb[kb][nb] = n < g.N && k2 < g.K ? Elem<T>::load(b + (g.b_mn ? k2 * g.ldb + n : n * g.ldb + k2)) : 0.f;
+__device__ __forceinline__ void write_row(uint32_t buf, int lane, const float (&v)[Out<T>::kCols]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint4 u;
+    if constexpr (sizeof(T) == 2) {
+      u.x = pack2(v[8 * j], v[8 * j + 1], (const T*)nullptr);
+      u.y = pack2(v[8 * j + 2], v[8 * j + 3], (const T*)nullptr);
+      u.z = pack2(v[8 * j + 4], v[8 * j + 5], (const T*)nullptr);
+      u.w = pack2(v[8 * j + 6], v[8 * j + 7], (const T*)nullptr);
+    } else {
+      u = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                     __float_as_uint(v[4 * j + 3]));
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += sa[k][ty * 4 + i] * sb[k][tx + 16 * j];
-    __syncthreads();
+    sts128(buf + lane * 128 + ((j ^ (lane & 7)) << 4), u);
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-      if (m >= g.M || n >= g.N) continue;
-      float z = acc[i][j];
-      if (g.bias) z += Elem<T>::load(static_cast<const T*>(g.bias) + n);
-      if (g.preact) Elem<T>::store(static_cast<T*>(g.preact) + m * g.N + n, z);
-      float y = act_value(z, g.act);
-      if (g.res) y += Elem<T>::load(static_cast<const T*>(g.res) + m * g.ldr + n);
-      Elem<T>::store(static_cast<T*>(g.out) + m * g.ldo + n, y);
+}
+template <typename T>
+__device__ __forceinline__ void add_row(uint32_t buf, int lane, float (&v)[Out<T>::kCols]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint4 u = lds128(buf + lane * 128 + ((j ^ (lane & 7)) << 4));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const float2 f = unpack2(w[i], (const T*)nullptr);
+        v[8 * j + 2 * i] += f.x;
+        v[8 * j + 2 * i + 1] += f.y;
+      } else {
+        v[4 * j + i] += __uint_as_float(w[i]);
+      }
+    }
+  }
+}
+// Rows the tensor engine cannot address: a warp copies its buffer element by element, a row's
+// columns side by side in the lanes.
+template <typename T, bool STORE>
+__device__ __forceinline__ void copy_rows(uint8_t* buf, T* g, int64_t ld, int rows, int cols, int lane) {
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int c = lane; c < Out<T>::kCols; c += 32) {
+      T* s = reinterpret_cast<T*>(buf + r * 128 + ((((c * (int)sizeof(T)) >> 4) ^ (r & 7)) << 4) +
+                                  ((c * (int)sizeof(T)) & 15));
+      if (c < cols) {
+        if (STORE) g[r * ld + c] = *s;
+        else *s = g[r * ld + c];
+      }
     }
 }
 
-size_t gemm_workspace(const Gemm&) { return 0; }
+// ---------------------------------------------------------------------------
+// the product
+// ---------------------------------------------------------------------------
+template <typename T, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    k_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res,
+              const __grid_constant__ CUtensorMap map_pre, const __grid_constant__ Args p) {
+  using L = Tile<BN>;
+  constexpr int kCols = Out<T>::kCols;
+  constexpr int kChunks = BN / kCols;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + L::OFF_BAR);
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
-murm_status gemm(const Gemm& g, void*, cudaStream_t st) {
-  const dim3 grid((g.N + 63) / 64, (g.M + 63) / 64);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->acc_full[i], 1);
+      mbar_init(&bars->acc_free[i], 2 * kEpiWarps);
+      for (int w = 0; w < kEpiWarps; ++w) {
+        mbar_init(&bars->res_full[w][i], 1);
+        mbar_init(&bars->res_free[w][i], 1);
+      }
+    }
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc_pair(&bars->tmem, L::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are up before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  pdl_wait();
+  pdl_trigger();
+
+  auto tile_of = [&](int item, int& m0, int& n0, int& split, int& i0, int& i1) {
+    split = item / p.tiles;
+    const int t = item - split * p.tiles;
+    m0 = (t / p.tiles_n) * 256;
+    n0 = (t % p.tiles_n) * BN;
+    i0 = split * p.iters;
+    i1 = min(p.total, i0 + p.iters);
+  };
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------ operand loads
+    int it = 0;
+    bool ok = true;
+    for (int item = first; ok && item < p.items; item += step) {
+      int m0, n0, split, i0, i1;
+      tile_of(item, m0, n0, split, i0, i1);
+      const int ma = m0 + (int)rank * 128, nb = n0 + (int)rank * (BN / 2);
+      for (int i = i0; i < i1; ++i, ++it) {
+        const int s = it % L::kStages;
+        if (!(ok = wait(&bars->empty[s], ((it / L::kStages) & 1) ^ 1))) break;
+        if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
+        const uint32_t bar = map_to_first(&bars->full[s]);
+        const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
+        const int pair = p.fp32 ? i / p.kblocks : 0;
+        const int k = (i - pair * p.kblocks) * kBK;
+        const int pa = p.fp32 ? plane_a(pair) : 0, pb = p.fp32 ? plane_b(pair) : 0;
+        if (p.a_mn) {
+          tma_load_pair(sa, &map_a, ma, k, pa, bar);
+          tma_load_pair(sa + 8192, &map_a, ma + 64, k, pa, bar);
+        } else {
+          tma_load_pair(sa, &map_a, k, ma, pa, bar);
+        }
+        if (p.b_mn) {
+#pragma unroll
+          for (int c = 0; c < BN / 128; ++c) tma_load_pair(sb + c * 8192, &map_b, nb + c * 64, k, pb, bar);
+        } else {
+          tma_load_pair(sb, &map_b, k, nb, pb, bar);
+        }
+      }
+    }
+    // the last stages' loads and releases must have arrived before the CTAs may exit
+    for (int j = it > L::kStages ? it - L::kStages : 0; j < it; ++j) {
+      const int s = j % L::kStages;
+      if (rank == 0 && !wait(&bars->full[s], (j / L::kStages) & 1)) break;
+      if (ok) ok = wait(&bars->empty[s], (j / L::kStages) & 1);
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ------------------------------------------------------------ MMAs of both CTAs
+    int it = 0, t = 0;
+    bool ok = true;
+    for (int item = first; ok && item < p.items; item += step, ++t) {
+      int m0, n0, split, i0, i1;
+      tile_of(item, m0, n0, split, i0, i1);
+      const int buf = t & 1;
+      if (!(ok = wait(&bars->acc_free[buf], ((t >> 1) & 1) ^ 1))) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * BN;
+      for (int i = i0; i < i1; ++i, ++it) {
+        const int s = it % L::kStages;
+        if (!(ok = wait(&bars->full[s], (it / L::kStages) & 1))) break;
+        tc_fence_after();
+        const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
+#pragma unroll
+        for (int kk = 0; kk < kBK / 16; ++kk) {
+          // K-major: 16 of a row's 64; MN-major: 16 of 64 rows, 64-wide column blocks 8 KB apart
+          const uint64_t da = p.a_mn ? smem_desc(sa + kk * 2048, 8192, 1024, kSwizzle128B)
+                                     : smem_desc(sa + kk * 32, 16, 1024, kSwizzle128B);
+          const uint64_t db = p.b_mn ? smem_desc(sb + kk * 2048, 8192, 1024, kSwizzle128B)
+                                     : smem_desc(sb + kk * 32, 16, 1024, kSwizzle128B);
+          mma_pair(d, da, db, p.idesc, i > i0 || kk > 0);
+        }
+        commit_pair(&bars->empty[s]);
+      }
+      if (ok) commit_pair(&bars->acc_full[buf]);
+    }
+  } else if (warp == 3 && lane == 0 && p.res && p.res_tma) {
+    // ------------------------------------------------------------ residual tiles
+    int q = 0;  // chunks loaded per warp
+    bool ok = true;
+    for (int item = first; ok && item < p.items; item += step) {
+      int m0, n0, split, i0, i1;
+      tile_of(item, m0, n0, split, i0, i1);
+      for (int c = 0; ok && c < kChunks && n0 + c * kCols < p.N; ++c, ++q)
+        for (int w = 0; w < kEpiWarps; ++w) {  // rows past M load as zeros
+          const int row = m0 + (int)rank * 128 + w * 32;
+          if (!(ok = wait(&bars->res_free[w][q & 1], ((q >> 1) & 1) ^ 1))) break;
+          mbar_arrive_expect_tx(&bars->res_full[w][q & 1], kBuf);
+          tma_load_2d(sbase + L::OFF_RES + (w * 2 + (q & 1)) * kBuf, &map_res, n0 + c * kCols, row,
+                      &bars->res_full[w][q & 1]);
+        }
+    }
+    for (int j = q > 2 ? q - 2 : 0; ok && j < q; ++j)
+      for (int w = 0; ok && w < kEpiWarps; ++w) ok = wait(&bars->res_full[w][j & 1], (j >> 1) & 1);
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int w = warp & 3;
+    const uint32_t out_buf = sbase + L::OFF_OUT + w * 2 * kBuf, res_buf = sbase + L::OFF_RES + w * 2 * kBuf;
+    uint8_t* out_ptr = smem + L::OFF_OUT + w * 2 * kBuf;
+    float* s_bias = reinterpret_cast<float*>(smem + L::OFF_BIAS) + w * 64;
+    int t = 0, stores = 0, q = 0;
+    bool ok = true;
+    const bool same_way = !p.pre || p.pre_tma == p.out_tma;  // stores alternate between the buffers
+    const bool any_tma = p.out_tma || (p.pre && p.pre_tma);
+    // stages a buffer's rows and sends them out
+    auto send = [&](const float(&v)[kCols], const CUtensorMap* map, int tma, T* base, int64_t ld, int row, int n,
+                    int store_row) {
+      const int b = stores++ & 1;
+      if (any_tma) {  // the buffer's last store has read it
+        if (lane == 0) {
+          if (same_way) tma_store_wait_read<1>();
+          else tma_store_wait_read<0>();
+        }
+        __syncwarp();
+      }
+      write_row<T>(out_buf + b * kBuf, lane, v);
+      if (tma) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tma_store_2d(map, out_buf + b * kBuf, n, store_row);
+      } else {
+        __syncwarp();
+        copy_rows<T, true>(out_ptr + b * kBuf, base + (int64_t)row * ld + n, ld, min(32, p.M - row), p.N - n, lane);
+        __syncwarp();
+      }
+    };
+    for (int item = first; ok && item < p.items; item += step, ++t) {
+      int m0, n0, split, i0, i1;
+      tile_of(item, m0, n0, split, i0, i1);
+      const int buf = t & 1;
+      const int row = m0 + (int)rank * 128 + w * 32;
+      ok = wait(&bars->acc_full[buf], (t >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * BN + ((uint32_t)(w * 32) << 16);
+      for (int c = 0; c < kChunks; ++c) {
+        const int n = n0 + c * kCols;
+        if (n >= p.N) break;
+        if (p.res && p.res_tma && row >= p.M) {  // its buffer turns over all the same
+          ok = wait(&bars->res_full[w][q & 1], (q >> 1) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->res_free[w][q & 1]);
+        }
+        if (row < p.M) {
+          float v[kCols];
+          if (p.bias) {
+            __syncwarp();
+            for (int j = lane; j < kCols; j += 32)
+              s_bias[j] = n + j < p.N ? Elem<T>::load(static_cast<const T*>(p.bias) + n + j) : 0.f;
+          }
+#pragma unroll
+          for (int h = 0; h < kCols / 32; ++h)
+            tmem_ld32(acc + c * kCols + h * 32, *reinterpret_cast<float(*)[32]>(&v[h * 32]));
+          tmem_wait_ld();
+          if (p.bias) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kCols; j += 4) {
+              const float4 bv = *reinterpret_cast<const float4*>(s_bias + j);
+              v[j] += bv.x; v[j + 1] += bv.y; v[j + 2] += bv.z; v[j + 3] += bv.w;
+            }
+          }
+          if (p.pre) send(v, &map_pre, p.pre_tma, static_cast<T*>(p.pre), p.N, row, n, row);
+          switch (p.act) {  // one loop per activation, so that the choice is made once per chunk
+            case MURM_ACT_NONE: break;
+            case MURM_ACT_RELU:
+#pragma unroll
+              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_RELU);
+              break;
+            case MURM_ACT_SILU:
+#pragma unroll
+              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_SILU);
+              break;
+            case MURM_ACT_GELU:
+#pragma unroll
+              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_GELU);
+              break;
+            default:
+#pragma unroll
+              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_GELU_TANH);
+          }
+          if (p.res) {
+            if (p.res_tma) {
+              const int b = q & 1;
+              ok = wait(&bars->res_full[w][b], (q >> 1) & 1);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              add_row<T>(res_buf + b * kBuf, lane, v);
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars->res_free[w][b]);
+            } else {
+              const T* res = static_cast<const T*>(p.res) + (int64_t)row * p.ldr + n;
+              copy_rows<T, false>(smem + L::OFF_RES + w * 2 * kBuf, const_cast<T*>(res), p.ldr, min(32, p.M - row),
+                                  p.N - n, lane);
+              __syncwarp();
+              add_row<T>(res_buf, lane, v);
+              __syncwarp();
+            }
+          }
+          send(v, &map_out, p.out_tma, static_cast<T*>(p.out), p.ldo, row, n, split * p.split_rows + row);
+        }
+        ++q;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(map_to_first(&bars->acc_free[buf]));
+    }
+    if (lane == 0) tma_store_wait_read<0>();
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no arrival, load or MMA of the pair is outstanding past this point
+  tc_fence_after();
+  if (warp == 2) tmem_free_pair(tmem, L::kTmemCols);
+}
+
+// out = epilogue of the K splits' sums, added in order. Four columns per thread.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_split_sum(const float* part, int64_t split_stride, int ldp, const __grid_constant__ Args p) {
+  pdl_wait();
+  const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+  const int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (n >= p.N || m >= p.M) return;
+  const float* src = part + m * ldp + n;
+  float4 s = *reinterpret_cast<const float4*>(src);
+  for (int i = 1; i < p.splits; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(src + i * split_stride);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  float z[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (n + j >= p.N) break;
+    if (p.bias) z[j] += Elem<T>::load(static_cast<const T*>(p.bias) + n + j);
+    if (p.pre) Elem<T>::store(static_cast<T*>(p.pre) + m * p.N + n + j, z[j]);
+    float y = act_value<Out<T>::kFast>(z[j], p.act);
+    if (p.res) y += Elem<T>::load(static_cast<const T*>(p.res) + m * p.ldr + n + j);
+    Elem<T>::store(static_cast<T*>(p.out) + m * p.ldo + n + j, y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// packing
+// ---------------------------------------------------------------------------
+// Eight columns per thread; dst rows of `pitch` elements, the columns past `cols` zero.
+template <typename T>
+__global__ void __launch_bounds__(256) k_pack(const T* src, int64_t ld, int64_t rows, int cols, uint16_t* dst, int pitch,
+                                              int64_t plane, int vec) {
+  pdl_wait();
+  const int64_t groups = (int64_t)rows * (pitch / 8);
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < groups; i += gridDim.x * 256ll) {
+    const int64_t r = i / (pitch / 8);
+    const int c = (int)(i - r * (pitch / 8)) * 8;
+    const T* s = src + r * ld + c;
+    alignas(16) uint16_t o[3][8];
+    if constexpr (sizeof(T) == 4) {
+      float v[8];
+      if (vec) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(s);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(s + 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? s[e] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint16_t t[3];
+        split3(v[e], t);
+        o[0][e] = t[0]; o[1][e] = t[1]; o[2][e] = t[2];
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<uint4*>(dst + q * plane + r * pitch + c) = *reinterpret_cast<const uint4*>(o[q]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[0][e] = c + e < cols ? *reinterpret_cast<const uint16_t*>(s + e) : 0;
+      *reinterpret_cast<uint4*>(dst + r * pitch + c) = *reinterpret_cast<const uint4*>(o[0]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+namespace {
+
+bool tma_rows(const void* p, int64_t ld, size_t es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0;
+}
+int64_t pitch_of(int cols) { return ((int64_t)cols + 7) / 8 * 8; }
+
+struct Config {
+  int bn, splits, iters, total, kblocks, tiles_m, tiles_n;
+};
+
+// Tile width and K splits by estimated time, in units of one stage of a 256-wide tile (512 clocks):
+// rounds of the pairs over the items times the item's stages plus its fill and drain.
+Config choose(const Gemm& g) {
+  Config best{};
+  double best_t = 0;
+  const int kblocks = (g.K + kBK - 1) / kBK;
+  const int total = kblocks * (g.a.planes == 3 ? 6 : 1);
+  for (int bn : {256, 128}) {
+    const int tm = (g.M + 255) / 256, tn = (g.N + bn - 1) / bn;
+    const int64_t tiles = (int64_t)tm * tn;
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (total / splits < 4 || tiles * splits > 2 * kPairs)) break;
+      const int iters = (total + splits - 1) / splits;
+      const int used = (total + iters - 1) / iters;
+      const int64_t rounds = (tiles * used + kPairs - 1) / kPairs;
+      double t = rounds * (iters * (bn / 256.0)) + 6;
+      if (used > 1) t += 8 + (double)g.M * g.N * 4 * (used + 1) / 1.5e6;
+      if (best_t == 0 || t < best_t) {
+        best_t = t;
+        best = Config{bn, used, iters, total, kblocks, tm, tn};
+      }
+    }
+  }
+  return best;
+}
+
+CUresult encode(CUtensorMap* map, CUtensorMapDataType type, size_t es, const void* p, int64_t cols, int64_t rows,
+                int64_t ld, int planes, int64_t plane, int box_cols, int box_rows) {
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * es), (cuuint64_t)((planes > 1 ? plane : ld) * es)};
+  cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+  cuuint32_t unit[3] = {1, 1, 1};
+  return tc_tensor_map_encoder()(map, type, planes ? 3 : 2, const_cast<void*>(p), dims, strides, box, unit,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == MURM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                           : dtype == MURM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+template <typename... KArgs, typename... Args>
+void launch(const char* name, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+            Args&&... args) {
+  MURM_LAUNCH_PDL(name, kernel, grid, threads, smem, st, args...);
+}
+
+template <typename T, int BN>
+murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t ldo, int64_t out_rows, int64_t out_cols,
+                      cudaStream_t st) {
+  const size_t es = sizeof(T);
+  constexpr int kCols = Out<T>::kCols;
+  const CUtensorMapDataType op = g.dtype == MURM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapDataType ot = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(g.dtype);
+  CUtensorMap ma, mb, mo{}, mr{}, mp{};
+  CUresult r;
+  if (g.a_mn) r = encode(&ma, op, 2, g.a.p, g.M, g.K, g.a.ld, g.a.planes, g.a.plane, 64, 64);
+  else r = encode(&ma, op, 2, g.a.p, g.K, g.M, g.a.ld, g.a.planes, g.a.plane, 64, 128);
+  if (r == CUDA_SUCCESS) {
+    if (g.b_mn) r = encode(&mb, op, 2, g.b.p, g.N, g.K, g.b.ld, g.b.planes, g.b.plane, 64, 64);
+    else r = encode(&mb, op, 2, g.b.p, g.K, g.N, g.b.ld, g.b.planes, g.b.plane, 64, BN / 2);
+  }
+  p.out = out;
+  p.ldo = ldo;
+  p.out_tma = tma_rows(out, ldo, es);
+  if (r == CUDA_SUCCESS && p.out_tma) r = encode(&mo, ot, es, out, out_cols, out_rows, ldo, 0, 0, kCols, 32);
+  if (p.res) {
+    p.res_tma = tma_rows(p.res, p.ldr, es);
+    if (r == CUDA_SUCCESS && p.res_tma) r = encode(&mr, ot, es, p.res, g.N, g.M, p.ldr, 0, 0, kCols, 32);
+  }
+  if (p.pre) {
+    p.pre_tma = tma_rows(p.pre, g.N, es);
+    if (r == CUDA_SUCCESS && p.pre_tma) r = encode(&mp, ot, es, p.pre, g.N, g.M, g.N, 0, 0, kCols, 32);
+  }
+  if (r != CUDA_SUCCESS) {
+    char msg[96];
+    snprintf(msg, sizeof msg, "linear: a tensor map was refused (%d)", (int)r);
+    return report_error(MURM_ERR_CUDA, msg);
+  }
+  const int items = p.items;
+  const int grid = 2 * (items < kPairs ? items : kPairs);
+  if (cudaError_t e = smem_opt_in(k_gemm_tc<T, BN>, Tile<BN>::kSmem))
+    return report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
+  launch("linear_gemm", k_gemm_tc<T, BN>, dim3(grid), kThreads, Tile<BN>::kSmem, st, ma, mb, mo, mr, mp, p);
+  return MURM_OK;
+}
+
+template <typename T>
+murm_status run(const Gemm& g, const Config& c, void* workspace, cudaStream_t st) {
+  Args p{};
+  p.M = g.M; p.N = g.N;
+  p.kblocks = c.kblocks; p.iters = c.iters; p.total = c.total; p.splits = c.splits;
+  p.tiles_n = c.tiles_n;
+  p.tiles = c.tiles_m * c.tiles_n;
+  p.items = p.tiles * c.splits;
+  p.idesc = idesc_f16(g.dtype == MURM_F16 ? 0 : 1, 256, c.bn, g.a_mn, g.b_mn);
+  p.a_mn = g.a_mn; p.b_mn = g.b_mn;
+  p.fp32 = g.a.planes == 3;
+  p.bias = g.bias; p.act = g.act;
+  p.res = g.res; p.ldr = g.ldr;
+  p.pre = g.preact;
+  murm_status s;
+  if (c.splits == 1) {
+    s = c.bn == 256 ? launch_tc<T, 256>(g, c, p, g.out, g.ldo, g.M, g.N, st)
+                    : launch_tc<T, 128>(g, c, p, g.out, g.ldo, g.M, g.N, st);
+  } else {
+    Args q = p;  // partial sums alone
+    q.bias = q.res = nullptr;
+    q.pre = nullptr;
+    q.act = MURM_ACT_NONE;
+    const int rows = c.tiles_m * 256, cols = c.tiles_n * c.bn;
+    q.M = rows;
+    q.N = cols;
+    q.split_rows = rows;
+    s = c.bn == 256 ? launch_tc<float, 256>(g, c, q, workspace, cols, (int64_t)rows * c.splits, cols, st)
+                    : launch_tc<float, 128>(g, c, q, workspace, cols, (int64_t)rows * c.splits, cols, st);
+    if (s == MURM_OK) {
+      p.out = g.out;
+      p.ldo = g.ldo;
+      launch("linear_split_sum", k_split_sum<T>, dim3((g.N + 255) / 256, (g.M + 3) / 4), 256, 0, st,
+             static_cast<const float*>(workspace), (int64_t)rows * cols, cols, p);
+    }
+  }
+  if (s != MURM_OK) return s;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MURM_OK : report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace
+
+size_t gemm_workspace(const Gemm& g) {
+  const Config c = choose(g);
+  return c.splits == 1 ? 0 : (size_t)c.splits * c.tiles_m * 256 * c.tiles_n * c.bn * sizeof(float);
+}
+
+murm_status gemm(const Gemm& g, void* workspace, cudaStream_t st) {
+  if (!tc_tensor_map_encoder()) return report_error(MURM_ERR_CUDA, "linear: cuTensorMapEncodeTiled is not available");
+  const Config c = choose(g);
   switch (g.dtype) {
-    case MURM_F32: MURM_LAUNCH("linear_gemm", k_gemm<float>, grid, 256, 0, st, g); break;
-    case MURM_F16: MURM_LAUNCH("linear_gemm", k_gemm<__half>, grid, 256, 0, st, g); break;
-    default: MURM_LAUNCH("linear_gemm", k_gemm<__nv_bfloat16>, grid, 256, 0, st, g);
+    case MURM_F32: return run<float>(g, c, workspace, st);
+    case MURM_F16: return run<__half>(g, c, workspace, st);
+    default: return run<__nv_bfloat16>(g, c, workspace, st);
+  }
+}
+
+bool needs_pack(int dtype, const Matrix& m) { return dtype == MURM_F32 || !tma_rows(m.p, m.ld, 2); }
+
+size_t pack_bytes(int dtype, const Matrix& m) {
+  return (size_t)m.rows * pitch_of(m.cols) * 2 * (dtype == MURM_F32 ? 3 : 1);
+}
+
+Operand packed_at(int dtype, const Matrix& m, void* dst) {
+  return Operand{dst, pitch_of(m.cols), m.rows * pitch_of(m.cols), dtype == MURM_F32 ? 3 : 1};
+}
+
+murm_status pack(int dtype, const Matrix& m, void* dst, cudaStream_t st) {
+  const int pitch = (int)pitch_of(m.cols);
+  const int64_t plane = m.rows * pitch;
+  int64_t blocks = (m.rows * (pitch / 8) + 255) / 256;
+  if (blocks > kSms * 16) blocks = kSms * 16;
+  if (dtype == MURM_F32) {
+    const int vec = m.cols % 8 == 0 && tma_rows(m.p, m.ld, 4);
+    launch("linear_pack", k_pack<float>, dim3((unsigned)blocks), 256, 0, st, static_cast<const float*>(m.p), m.ld, m.rows,
+           m.cols, static_cast<uint16_t*>(dst), pitch, plane, vec);
+  } else {
+    launch("linear_pack", k_pack<__half>, dim3((unsigned)blocks), 256, 0, st, static_cast<const __half*>(m.p), m.ld,
+           m.rows, m.cols, static_cast<uint16_t*>(dst), pitch, plane, 0);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MURM_OK : report_error(MURM_ERR_CUDA, cudaGetErrorString(e));

@@ -32,12 +32,36 @@ constexpr int kDzChunks = 128;  // most row chunks, each with one partial of db
 
 template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T e[V]; };
 
-// Block (x, y): V * 32 columns, a chunk of rows; 8 warps take the chunk's rows in turn. dz is
-// rounded to T, the type its products take it in; db sums it unrounded, in fp32, a thread's rows in
-// order, then the block's 8 warps in order, then (k_col_sum) the chunks in order.
+// dz becomes the products' operand: rounded to T where that is 16 bits wide, three bf16 planes
+// that hold it exactly for fp32.
+template <typename T, int V>
+__device__ __forceinline__ void store_operand(const Operand& o, int64_t at, const float (&d)[V]) {
+  if constexpr (sizeof(T) == 2) {
+    Pack<T, V> r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) Elem<T>::store(r.e + e, d[e]);
+    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(const_cast<void*>(o.p)) + at) = r;
+  } else {
+    Pack<uint16_t, V> r[3];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      uint16_t t[3];
+      split3(d[e], t);
+      for (int q = 0; q < 3; ++q) r[q].e[e] = t[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      *reinterpret_cast<Pack<uint16_t, V>*>(static_cast<uint16_t*>(const_cast<void*>(o.p)) + q * o.plane + at) = r[q];
+  }
+}
+
+// Block (x, y): V * 32 columns, a chunk of rows; 8 warps take the chunk's rows in turn. db sums dz
+// unrounded, in fp32: a thread's rows in order, then the block's 8 warps in order, then (k_col_sum)
+// the chunks in order.
 template <typename T, int V>
 __global__ void __launch_bounds__(kDzCols * kDzRows)
-    k_dz(const T* dy, int64_t ldy, const T* z, int M, int N, int act, int chunk, T* dz, float* part) {
+    k_dz(const T* dy, int64_t ldy, const T* z, int M, int N, int act, int chunk,
+         Operand dz, float* part) {
   __shared__ float s[kDzRows][kDzCols * V + 1];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n = (blockIdx.x * kDzCols + tx) * V;
@@ -55,13 +79,9 @@ __global__ void __launch_bounds__(kDzCols * kDzRows)
       for (int e = 0; e < V; ++e) d[e] = Elem<T>::load(g.e + e);
       if (z) {
         const P zz = *reinterpret_cast<const P*>(z + (int64_t)m * N + n);
-        P o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          d[e] *= act_slope(Elem<T>::load(zz.e + e), act);
-          Elem<T>::store(o.e + e, d[e]);
-        }
-        if (dz) *reinterpret_cast<P*>(dz + (int64_t)m * N + n) = o;
+        for (int e = 0; e < V; ++e) d[e] *= act_slope<sizeof(T) == 2>(Elem<T>::load(zz.e + e), act);
+        if (dz.p) store_operand<T, V>(dz, (int64_t)m * dz.ld + n, d);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] += d[e];
@@ -106,7 +126,7 @@ int dz_chunks(int M, int N, int V) {
 }
 
 template <typename T, int V>
-void launch_dz(const murm_linear_bwd_args& a, T* dz, float* part, cudaStream_t st) {
+void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cudaStream_t st) {
   const int M = (int)a.rows, N = a.out_features;
   const int most = dz_chunks(M, N, V);
   const int chunk = (M + most - 1) / most;
@@ -121,13 +141,13 @@ void launch_dz(const murm_linear_bwd_args& a, T* dz, float* part, cudaStream_t s
 }
 
 template <typename T>
-void run_dz(const murm_linear_bwd_args& a, void* dz, float* part, cudaStream_t st) {
+void run_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a.grad_out) | reinterpret_cast<uintptr_t>(a.preact);
   if (a.out_features % V == 0 && a.go_stride % V == 0 && bits % 16 == 0)
-    launch_dz<T, V>(a, static_cast<T*>(dz), part, st);
+    launch_dz<T, V>(a, dz, part, st);
   else
-    launch_dz<T, 1>(a, static_cast<T*>(dz), part, st);
+    launch_dz<T, 1>(a, dz, part, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -191,61 +211,123 @@ murm_status check_ws(const void* ws, size_t have, size_t need) {
   return MURM_OK;
 }
 
-Gemm forward_gemm(const murm_linear_args& a) {
-  Gemm g{};
+// A matrix as an operand: in place where TMA can read it, else packed at an offset of the workspace.
+struct Source {
+  Matrix m;
+  bool packed;
+  size_t at;
+  Operand op;
+};
+struct Layout {
+  size_t bytes = 0;
+  char* ws;
+  int dtype;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += align256(n);
+    return at;
+  }
+  Source source(const void* p, int64_t ld, int64_t rows, int cols) {
+    Source s{Matrix{p, ld, rows, cols}, false, 0, {}};
+    s.packed = needs_pack(dtype, s.m);
+    if (s.packed) {
+      s.at = take(pack_bytes(dtype, s.m));
+      s.op = packed_at(dtype, s.m, ws + s.at);
+    } else {
+      s.op = Operand{p, ld, 0, 1};
+    }
+    return s;
+  }
+};
+murm_status fill(const Source& s, const Layout& l, cudaStream_t st) {
+  return s.packed ? pack(l.dtype, s.m, l.ws + s.at, st) : MURM_OK;
+}
+
+struct FwdPlan {
+  Layout l;
+  Source x, w;
+  Gemm g;
+  size_t gemm_at;
+};
+FwdPlan plan_fwd(const murm_linear_args& a) {
+  FwdPlan p{};
+  p.l.ws = static_cast<char*>(a.workspace);
+  p.l.dtype = a.dtype;
+  p.x = p.l.source(a.x, a.x_stride, a.rows, a.in_features);
+  p.w = p.l.source(a.weight, a.w_stride, a.out_features, a.in_features);
+  Gemm& g = p.g;
   g.dtype = a.dtype;
-  g.a = a.x; g.lda = a.x_stride;
-  g.b = a.weight; g.ldb = a.w_stride;
+  g.a = p.x.op;
+  g.b = p.w.op;
   g.M = (int)a.rows; g.N = a.out_features; g.K = a.in_features;
   g.bias = a.bias;
   g.res = a.residual; g.ldr = a.r_stride;
   g.out = a.out; g.ldo = a.out_stride;
   g.preact = a.preact;
   g.act = a.activation;
-  return g;
+  p.gemm_at = p.l.take(gemm_workspace(g));
+  return p;
 }
 
-// dz as the products' operand: the pass's result, or grad_out itself without an activation.
 struct BwdPlan {
-  bool act, need_dz, need_db;
-  size_t dz_at, part_at, gemm_at, bytes;
+  Layout l;
+  bool act, products;
+  Source x, w, dy;  // dy: dz itself without an activation
+  Operand dz;
+  size_t part_at, gemm_at;
   Gemm gx, gw;
 };
 BwdPlan plan_bwd(const murm_linear_bwd_args& a) {
   BwdPlan p{};
+  p.l.ws = static_cast<char*>(a.workspace);
+  p.l.dtype = a.dtype;
   p.act = a.activation != MURM_ACT_NONE;
-  p.need_dz = p.act && (a.grad_x || a.grad_weight);
-  p.need_db = a.grad_bias != nullptr;
-  size_t o = 0;
-  auto take = [&o](size_t n) { const size_t at = o; o += align256(n); return at; };
-  p.dz_at = take(p.need_dz ? (size_t)a.rows * a.out_features * elem_size(a.dtype) : 0);
-  p.part_at = take(p.need_db ? (size_t)kDzChunks * a.out_features * sizeof(float) : 0);
-  p.gemm_at = o;
-  const char* ws = static_cast<const char*>(a.workspace);
-  const void* dz = p.act ? ws + p.dz_at : a.grad_out;
-  const int64_t ldz = p.act ? a.out_features : a.go_stride;
+  p.products = a.grad_x || a.grad_weight;
+  if (p.products) {
+    if (p.act) {
+      const Matrix m{nullptr, 0, a.rows, a.out_features};
+      const size_t at = p.l.take(pack_bytes(a.dtype, m));
+      p.dz = packed_at(a.dtype, m, p.l.ws + at);
+    } else {
+      p.dy = p.l.source(a.grad_out, a.go_stride, a.rows, a.out_features);
+      p.dz = p.dy.op;
+    }
+  }
+  if (a.grad_x) p.w = p.l.source(a.weight, a.w_stride, a.out_features, a.in_features);
+  if (a.grad_weight) p.x = p.l.source(a.x, a.x_stride, a.rows, a.in_features);
+  p.part_at = p.l.take(a.grad_bias ? (size_t)kDzChunks * a.out_features * sizeof(float) : 0);
   Gemm g{};
   g.dtype = a.dtype;
-  g.a = dz; g.lda = ldz;
+  g.a = p.dz;
+  g.N = a.in_features;
+  g.b_mn = true;
   size_t most = 0;
   if (a.grad_x) {
     p.gx = g;
-    p.gx.b = a.weight; p.gx.ldb = a.w_stride; p.gx.b_mn = true;
-    p.gx.M = (int)a.rows; p.gx.N = a.in_features; p.gx.K = a.out_features;
+    p.gx.b = p.w.op;
+    p.gx.M = (int)a.rows; p.gx.K = a.out_features;
     p.gx.out = a.grad_x; p.gx.ldo = a.gx_stride;
     most = gemm_workspace(p.gx);
   }
   if (a.grad_weight) {
     p.gw = g;
     p.gw.a_mn = true;
-    p.gw.b = a.x; p.gw.ldb = a.x_stride; p.gw.b_mn = true;
-    p.gw.M = a.out_features; p.gw.N = a.in_features; p.gw.K = (int)a.rows;
+    p.gw.b = p.x.op;
+    p.gw.M = a.out_features; p.gw.K = (int)a.rows;
     p.gw.out = a.grad_weight; p.gw.ldo = a.gw_stride;
     const size_t w = gemm_workspace(p.gw);
     most = w > most ? w : most;
   }
-  p.bytes = p.gemm_at + most;
+  p.gemm_at = p.l.take(most);
   return p;
+}
+
+murm_status run_fwd(const murm_linear_args& a, cudaStream_t st) {
+  const FwdPlan p = plan_fwd(a);
+  if (murm_status s = check_ws(a.workspace, a.workspace_bytes, p.l.bytes)) return s;
+  if (murm_status s = fill(p.x, p.l, st)) return s;
+  if (murm_status s = fill(p.w, p.l, st)) return s;
+  return gemm(p.g, p.l.ws + p.gemm_at, st);
 }
 
 murm_status run_bwd(const murm_linear_bwd_args& a, cudaStream_t st) {
@@ -258,11 +340,10 @@ murm_status run_bwd(const murm_linear_bwd_args& a, cudaStream_t st) {
     return e == cudaSuccess ? MURM_OK : bad(MURM_ERR_CUDA, "clearing gradients: %s", cudaGetErrorString(e));
   }
   const BwdPlan p = plan_bwd(a);
-  if (murm_status s = check_ws(a.workspace, a.workspace_bytes, p.bytes)) return s;
-  char* ws = static_cast<char*>(a.workspace);
-  if (p.need_dz || p.need_db) {
-    void* dz = p.need_dz ? ws + p.dz_at : nullptr;
-    float* part = p.need_db ? reinterpret_cast<float*>(ws + p.part_at) : nullptr;
+  if (murm_status s = check_ws(a.workspace, a.workspace_bytes, p.l.bytes)) return s;
+  if ((p.act && p.products) || a.grad_bias) {
+    const Operand dz = p.act ? p.dz : Operand{};
+    float* part = a.grad_bias ? reinterpret_cast<float*>(p.l.ws + p.part_at) : nullptr;
     switch (a.dtype) {
       case MURM_F32: run_dz<float>(a, dz, part, st); break;
       case MURM_F16: run_dz<__half>(a, dz, part, st); break;
@@ -271,10 +352,13 @@ murm_status run_bwd(const murm_linear_bwd_args& a, cudaStream_t st) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return bad(MURM_ERR_CUDA, "linear backward launch: %s", cudaGetErrorString(e));
   }
+  if (murm_status s = fill(p.dy, p.l, st)) return s;
+  if (murm_status s = fill(p.w, p.l, st)) return s;
+  if (murm_status s = fill(p.x, p.l, st)) return s;
   if (a.grad_x)
-    if (murm_status s = gemm(p.gx, ws + p.gemm_at, st)) return s;
+    if (murm_status s = gemm(p.gx, p.l.ws + p.gemm_at, st)) return s;
   if (a.grad_weight)
-    if (murm_status s = gemm(p.gw, ws + p.gemm_at, st)) return s;
+    if (murm_status s = gemm(p.gw, p.l.ws + p.gemm_at, st)) return s;
   return MURM_OK;
 }
 
@@ -289,20 +373,18 @@ extern "C" {
 murm_status murm_linear_workspace(const murm_linear_args* args, size_t* bytes) {
   if (!bytes) return bad(MURM_ERR_INVALID_ARGUMENT, "bytes is NULL");
   if (murm_status s = check_fwd(args)) return s;
-  *bytes = args->rows ? gemm_workspace(forward_gemm(*args)) : 0;
+  *bytes = args->rows ? plan_fwd(*args).l.bytes : 0;
   return MURM_OK;
 }
 murm_status murm_linear_fwd(const murm_linear_args* args, void* stream) {
   if (murm_status s = check_fwd(args)) return s;
   if (args->rows == 0) return MURM_OK;
-  const Gemm g = forward_gemm(*args);
-  if (murm_status s = check_ws(args->workspace, args->workspace_bytes, gemm_workspace(g))) return s;
-  return gemm(g, args->workspace, static_cast<cudaStream_t>(stream));
+  return run_fwd(*args, static_cast<cudaStream_t>(stream));
 }
 murm_status murm_linear_bwd_workspace(const murm_linear_bwd_args* args, size_t* bytes) {
   if (!bytes) return bad(MURM_ERR_INVALID_ARGUMENT, "bytes is NULL");
   if (murm_status s = check_bwd(args)) return s;
-  *bytes = args->rows ? plan_bwd(*args).bytes : 0;
+  *bytes = args->rows ? plan_bwd(*args).l.bytes : 0;
   return MURM_OK;
 }
 murm_status murm_linear_bwd(const murm_linear_bwd_args* args, void* stream) {

@@ -1,4 +1,4 @@
-// murm_linear.cuh — the matrix product of the linear layer: description, epilogue math, entry.
+// murm_linear.cuh — the matrix product of the linear layer: description, epilogue math, entries.
 #pragma once
 
 #include "murm_kernels.cuh"
@@ -6,12 +6,21 @@
 namespace murm {
 namespace lin {
 
-// D[m][n] = sum over k of A(m,k) B(n,k); z = D + bias[n]; out = act(z) + residual[m][n].
-// A is a[m*lda + k], or with a_mn a[k*lda + m]; B likewise.
+// A 16-bit matrix the tensor cores read through TMA: row-major [rows][cols] with a row stride of
+// `ld` elements (a multiple of 8; base 16-byte aligned). fp32 data is three bf16 planes, `plane`
+// elements apart, that add up to it exactly.
+struct Operand {
+  const void* p;
+  int64_t ld, plane;
+  int planes;
+};
+
+// D(m,n) = sum over k of A(m,k) B(n,k); z = D + bias[n]; out = act(z) + residual(m,n).
+// The operand's rows are m (n) and its columns k; with a_mn (b_mn) its rows are k.
 struct Gemm {
-  int dtype;  // of a, b, out and the epilogue's tensors
-  const void* a; int64_t lda; bool a_mn;
-  const void* b; int64_t ldb; bool b_mn;
+  int dtype;  // murm_dtype of out and of the epilogue's tensors
+  Operand a, b;
+  bool a_mn, b_mn;
   int M, N, K;
   const void* bias;
   const void* res; int64_t ldr;
@@ -22,41 +31,106 @@ struct Gemm {
 size_t gemm_workspace(const Gemm& g);
 murm_status gemm(const Gemm& g, void* workspace, cudaStream_t st);
 
+// Packing of a row-major matrix into an Operand: fp32 always (three planes), 16-bit data when its
+// address or stride is not one TMA can take.
+struct Matrix {
+  const void* p;
+  int64_t ld;
+  int64_t rows;
+  int cols;
+};
+bool needs_pack(int dtype, const Matrix& m);
+size_t pack_bytes(int dtype, const Matrix& m);
+Operand packed_at(int dtype, const Matrix& m, void* dst);  // the operand pack() writes at dst
+murm_status pack(int dtype, const Matrix& m, void* dst, cudaStream_t st);
+
 // ---------------------------------------------------------------------------
 // activations, in fp32
 // ---------------------------------------------------------------------------
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kSqrt2OverPi = 0.79788456080286536f;
+constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float sigmoidf_(float x) { return 1.f / (1.f + expf(-x)); }
+// FAST: for results rounded to 16 bits, with the hardware's exp2 and reciprocal (relative errors
+// near 2^-22); else CUDA's accurate functions.
+template <bool FAST>
+__device__ __forceinline__ float exp_(float x) {
+  if (!FAST) return expf(x);
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * kLog2e));
+  return r;
+}
+template <bool FAST>
+__device__ __forceinline__ float rcp_(float x) {
+  if (!FAST) return 1.f / x;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_(float x) { return rcp_<FAST>(1.f + exp_<FAST>(-x)); }
 
+// The standard normal distribution function. FAST: 0.5 erfc(|z| / sqrt 2) by formula 7.1.26 of
+// Abramowitz and Stegun (absolute error of erf at most 1.5e-7), with the argument's 1/sqrt 2 and
+// the result's 1/2 folded into the coefficients.
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float z) {
+  if (!FAST) return 0.5f * (1.f + erff(z * kSqrtHalf));
+  const float a = fabsf(z);
+  const float t = rcp_<true>(fmaf(0.3275911f * kSqrtHalf, a, 1.f));
+  float q = fmaf(t, 0.5f * 1.061405429f, -0.5f * 1.453152027f);
+  q = fmaf(q, t, 0.5f * 1.421413741f);
+  q = fmaf(q, t, -0.5f * 0.284496736f);
+  q = fmaf(q, t, 0.5f * 0.254829592f);
+  q *= t * exp_<true>(-0.5f * z * z);
+  return z < 0.f ? q : 1.f - q;  // NaN: q is NaN
+}
+
+template <bool FAST>
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case MURM_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps NaN
-    case MURM_ACT_SILU: return z * sigmoidf_(z);
-    case MURM_ACT_GELU: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+    case MURM_ACT_SILU: return z * sigmoid_<FAST>(z);
+    case MURM_ACT_GELU: return z * normal_cdf<FAST>(z);
     case MURM_ACT_GELU_TANH:  // 0.5 (1 + tanh u) = sigmoid(2u)
-      return z * sigmoidf_(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
+      return z * sigmoid_<FAST>(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
   }
   return z;
 }
 // d act / dz
+template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case MURM_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case MURM_ACT_SILU: {
-      const float s = sigmoidf_(z);
+      const float s = sigmoid_<FAST>(z);
       return s * (1.f + z * (1.f - s));
     }
-    case MURM_ACT_GELU:
-      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expf(-0.5f * z * z);
+    case MURM_ACT_GELU: return normal_cdf<FAST>(z) + z * kInvSqrt2Pi * exp_<FAST>(-0.5f * z * z);
     case MURM_ACT_GELU_TANH: {
-      const float s = sigmoidf_(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
+      const float s = sigmoid_<FAST>(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
       return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * 0.044715f * z * z);
     }
   }
   return 1.f;
+}
+
+// The three bf16 terms of an fp32 value, each the leading 8 bits of what is left (cut, so that no
+// term overflows): they add up to it exactly, as long as the last stays above bf16's smallest
+// number. Infinities and NaN go to the first term alone.
+__device__ __forceinline__ void split3(float x, uint16_t (&t)[3]) {
+  const uint32_t u = __float_as_uint(x);
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    t[0] = (u & 0x007fffffu) ? 0x7fffu : (uint16_t)(u >> 16);
+    t[1] = t[2] = 0;
+    return;
+  }
+  t[0] = (uint16_t)(u >> 16);
+  const float r = x - __uint_as_float(u & 0xffff0000u);
+  const uint32_t v = __float_as_uint(r);
+  t[1] = (uint16_t)(v >> 16);
+  t[2] = (uint16_t)(__float_as_uint(r - __uint_as_float(v & 0xffff0000u)) >> 16);
 }
 
 }  // namespace lin
