@@ -7,10 +7,10 @@
 // k_gemm_tc: a pair of CTAs (cta_group::2) per 256 x BN tile, each holding 128 rows of A, half the
 // rows of B and a 128 x BN fp32 accumulator in TMEM (two accumulators: a tile's epilogue runs under
 // the next tile's products). Persistent over the tiles. Warp 0 loads the operands by TMA into a
-// ring of 64-deep stages, warp 1 of the first CTA issues the MMAs of both, warp 3 loads residual
-// tiles, warps 4-7 run the epilogue: TMEM -> registers -> bias, activation, residual -> 128-byte
-// swizzled rows in shared memory -> TMA store (or plain stores where the result's rows are not
-// 16-byte aligned).
+// ring of 64-deep stages, warp 1 of the first CTA issues the MMAs of both, warps 4-11 run the
+// epilogue, each on 32 rows and half the columns: TMEM -> registers -> bias, activation, residual ->
+// 128-byte swizzled rows in shared memory -> TMA store (or plain stores where the result's rows are
+// not 16-byte aligned).
 //
 // fp32 operands are three bf16 planes; the products of planes (i, j) with i + j <= 2 carry them to
 // 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K
@@ -36,41 +36,38 @@ constexpr int kSms = 148;
 constexpr int kPairs = kSms / 2;     // CTA pairs resident at once
 constexpr int kBK = 64;              // depth of a stage: one 128-byte swizzled row
 constexpr uint32_t kABytes = 128 * kBK * 2;
-constexpr int kEpiWarps = 4;
-constexpr int kThreads = 256;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr uint32_t kBuf = 32 * 128;  // one epilogue warp's 32 rows of 128 bytes
 
 template <int BN> struct Tile {
   static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
   static constexpr uint32_t kStage = kABytes + kBBytes;
-  static constexpr int kStages = BN == 256 ? 5 : 6;
-  static constexpr uint32_t OFF_OUT = kStages * kStage;            // [warp][2] result buffers
-  static constexpr uint32_t OFF_RES = OFF_OUT + kEpiWarps * 2 * kBuf;  // [warp][2] residual buffers
-  static constexpr uint32_t OFF_BIAS = OFF_RES + kEpiWarps * 2 * kBuf;
-  static constexpr uint32_t OFF_BAR = OFF_BIAS + kEpiWarps * 64 * 4;
-  static constexpr uint32_t kSmem = OFF_BAR + 512 + 1024;
+  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr uint32_t OFF_OUT = kStages * kStage;  // one buffer per epilogue warp
+  static constexpr uint32_t OFF_BAR = OFF_OUT + kEpiWarps * kBuf;
+  static constexpr uint32_t kSmem = OFF_BAR + 256 + 1024;
   static constexpr uint32_t kTmemCols = 2 * BN;
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 
 struct Bars {  // in shared memory at OFF_BAR
-  uint64_t full[8], empty[8];        // operand stages; `full` of the pair's first CTA counts both loads
+  uint64_t full[8], empty[8];         // operand stages; `full` of the pair's first CTA counts both loads
   uint64_t acc_full[2], acc_free[2];  // accumulators; acc_free is used in the pair's first CTA
-  uint64_t res_full[kEpiWarps][2], res_free[kEpiWarps][2];
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 512, "barrier area");
+static_assert(sizeof(Bars) <= 256, "barrier area");
 
 struct Args {
   int M, N;
-  int kblocks, iters, total, splits;  // stages per plane pair, per split, in all; K splits
-  int tiles_n, tiles, items;          // items: tiles * splits
+  int kblocks, iters, total, splits;      // stages per plane pair, per split, in all; K splits
+  int tiles_m, tiles_n, tiles, items;     // items: tiles * splits
   uint32_t idesc;
   int a_mn, b_mn;
   int fp32;  // operands are three planes
-  const void* bias;
+  const void* bias; int bias_vec;         // *_vec: 16-byte accesses are aligned and stay inside the row
   int act;
-  const void* res; int64_t ldr; int res_tma;
+  const void* res; int64_t ldr; int res_vec;
   void* out; int64_t ldo; int out_tma;
   void* pre; int pre_tma;
   int split_rows;  // rows of one split's partial result
@@ -109,13 +106,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -123,11 +113,8 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// All but the newest N of this thread's stores have read their shared memory.
-template <int N>
-__device__ __forceinline__ void tma_store_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
+// This thread's stores have read their shared memory.
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -230,8 +217,25 @@ __device__ __forceinline__ void add_row(uint32_t buf, int lane, float (&v)[Out<T
     }
   }
 }
-// Rows the tensor engine cannot address: a warp copies its buffer element by element, a row's
-// columns side by side in the lanes.
+// A warp's 32 rows of a buffer in global memory, eight lanes to a row: coalesced 16-byte accesses.
+template <typename T>
+__device__ __forceinline__ void load_rows(const T* g, int64_t ld, int rows, int cols, int lane, uint4 (&v)[8]) {
+  const int c = (lane & 7) * (16 / (int)sizeof(T));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (r < rows && c < cols) v[i] = __ldg(reinterpret_cast<const uint4*>(g + r * ld + c));
+  }
+}
+__device__ __forceinline__ void put_rows(uint32_t buf, int lane, const uint4 (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    sts128(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4), v[i]);
+  }
+}
+// The same rows where 16-byte accesses are not aligned: element by element, columns side by side.
 template <typename T, bool STORE>
 __device__ __forceinline__ void copy_rows(uint8_t* buf, T* g, int64_t ld, int rows, int cols, int lane) {
   for (int r = 0; r < rows; ++r)
@@ -245,18 +249,79 @@ __device__ __forceinline__ void copy_rows(uint8_t* buf, T* g, int64_t ld, int ro
       }
     }
 }
+// v += the bias of a chunk's columns: the same address in every lane, from L1.
+template <typename T>
+__device__ __forceinline__ void add_bias(const T* bias, int vec, int cols, float (&v)[Out<T>::kCols]) {
+  constexpr int kPer = 16 / sizeof(T);
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < Out<T>::kCols / kPer; ++j) {
+      if (j * kPer >= cols) break;
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias) + j);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[j * kPer + i] += Elem<T>::load(e + i);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < Out<T>::kCols; ++j)
+      if (j < cols) v[j] += Elem<T>::load(bias + j);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void activate(float (&v)[Out<T>::kCols], int act) {
+  constexpr bool F = Out<T>::kFast;
+  switch (act) {  // one loop per activation: the choice is made once
+    case MURM_ACT_NONE: break;
+    case MURM_ACT_RELU:
+#pragma unroll
+      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_RELU);
+      break;
+    case MURM_ACT_SILU:
+#pragma unroll
+      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_SILU);
+      break;
+    case MURM_ACT_GELU:
+#pragma unroll
+      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_GELU);
+      break;
+    default:
+#pragma unroll
+      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_GELU_TANH);
+  }
+}
 
 // ---------------------------------------------------------------------------
 // the product
 // ---------------------------------------------------------------------------
+struct Item {
+  int m0, n0, split, i0, i1;
+};
+// Tiles run down kGroupM tile rows before the next tile column, so that the tiles in flight at once
+// read few rows of A and few of B from L2.
+constexpr int kGroupM = 8;
+template <int BN>
+__device__ __forceinline__ Item item_at(const Args& p, int item) {
+  Item r;
+  r.split = item / p.tiles;
+  const int t = item - r.split * p.tiles;
+  const int g = t / (kGroupM * p.tiles_n), in = t - g * kGroupM * p.tiles_n;
+  const int gm = min(kGroupM, p.tiles_m - g * kGroupM);
+  const int n = in / gm;
+  r.m0 = (g * kGroupM + in - n * gm) * 256;
+  r.n0 = n * BN;
+  r.i0 = r.split * p.iters;
+  r.i1 = min(p.total, r.i0 + p.iters);
+  return r;
+}
+
 template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res,
-              const __grid_constant__ CUtensorMap map_pre, const __grid_constant__ Args p) {
+              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
+              const __grid_constant__ Args p) {
   using L = Tile<BN>;
   constexpr int kCols = Out<T>::kCols;
-  constexpr int kChunks = BN / kCols;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   Bars* bars = reinterpret_cast<Bars*>(smem + L::OFF_BAR);
@@ -273,10 +338,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->acc_full[i], 1);
       mbar_init(&bars->acc_free[i], 2 * kEpiWarps);
-      for (int w = 0; w < kEpiWarps; ++w) {
-        mbar_init(&bars->res_full[w][i], 1);
-        mbar_init(&bars->res_free[w][i], 1);
-      }
     }
     fence_barrier_init();
   }
@@ -289,31 +350,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  auto tile_of = [&](int item, int& m0, int& n0, int& split, int& i0, int& i1) {
-    split = item / p.tiles;
-    const int t = item - split * p.tiles;
-    m0 = (t / p.tiles_n) * 256;
-    n0 = (t % p.tiles_n) * BN;
-    i0 = split * p.iters;
-    i1 = min(p.total, i0 + p.iters);
-  };
-
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------ operand loads
-    int it = 0;
+    uint32_t s = 0, ph = 0;  // stage and its round's parity
+    int issued = 0;
     bool ok = true;
     for (int item = first; ok && item < p.items; item += step) {
-      int m0, n0, split, i0, i1;
-      tile_of(item, m0, n0, split, i0, i1);
-      const int ma = m0 + (int)rank * 128, nb = n0 + (int)rank * (BN / 2);
-      for (int i = i0; i < i1; ++i, ++it) {
-        const int s = it % L::kStages;
-        if (!(ok = wait(&bars->empty[s], ((it / L::kStages) & 1) ^ 1))) break;
+      const Item t = item_at<BN>(p, item);
+      const int ma = t.m0 + (int)rank * 128, nb = t.n0 + (int)rank * (BN / 2);
+      int pair = p.fp32 ? t.i0 / p.kblocks : 0;
+      int kb = t.i0 - pair * p.kblocks;
+      for (int i = t.i0; i < t.i1; ++i) {
+        if (!(ok = wait(&bars->empty[s], ph ^ 1))) break;
         if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
         const uint32_t bar = map_to_first(&bars->full[s]);
         const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
-        const int pair = p.fp32 ? i / p.kblocks : 0;
-        const int k = (i - pair * p.kblocks) * kBK;
+        const int k = kb * kBK;
         const int pa = p.fp32 ? plane_a(pair) : 0, pb = p.fp32 ? plane_b(pair) : 0;
         if (p.a_mn) {
           tma_load_pair(sa, &map_a, ma, k, pa, bar);
@@ -327,178 +379,123 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         } else {
           tma_load_pair(sb, &map_b, k, nb, pb, bar);
         }
+        ++issued;
+        if (++kb == p.kblocks) { kb = 0; ++pair; }
+        if (++s == L::kStages) { s = 0; ph ^= 1; }
       }
     }
     // the last stages' loads and releases must have arrived before the CTAs may exit
-    for (int j = it > L::kStages ? it - L::kStages : 0; j < it; ++j) {
-      const int s = j % L::kStages;
-      if (rank == 0 && !wait(&bars->full[s], (j / L::kStages) & 1)) break;
-      if (ok) ok = wait(&bars->empty[s], (j / L::kStages) & 1);
+    for (int j = max(0, issued - L::kStages); j < issued; ++j) {
+      const int st = j % L::kStages, par = (j / L::kStages) & 1;
+      if (rank == 0 && !wait(&bars->full[st], par)) break;
+      if (ok) ok = wait(&bars->empty[st], par);
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
     // ------------------------------------------------------------ MMAs of both CTAs
-    int it = 0, t = 0;
+    // Operand descriptors: K-major steps through 16 of a row's 64 elements (32 bytes), MN-major
+    // through 16 of 64 rows (2 KB), its 64-wide column blocks 8 KB apart. Only the low word, which
+    // holds the address, changes.
+    const uint64_t da = smem_desc(sbase, p.a_mn ? 8192 : 16, 1024, kSwizzle128B);
+    const uint64_t db = smem_desc(sbase + kABytes, p.b_mn ? 8192 : 16, 1024, kSwizzle128B);
+    const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
+    const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
+    uint32_t s = 0, ph = 0;
+    int t = 0;
     bool ok = true;
     for (int item = first; ok && item < p.items; item += step, ++t) {
-      int m0, n0, split, i0, i1;
-      tile_of(item, m0, n0, split, i0, i1);
+      const Item w = item_at<BN>(p, item);
       const int buf = t & 1;
       if (!(ok = wait(&bars->acc_free[buf], ((t >> 1) & 1) ^ 1))) break;
       tc_fence_after();
       const uint32_t d = tmem + buf * BN;
-      for (int i = i0; i < i1; ++i, ++it) {
-        const int s = it % L::kStages;
-        if (!(ok = wait(&bars->full[s], (it / L::kStages) & 1))) break;
+      uint32_t more = 0;
+      for (int i = w.i0; i < w.i1; ++i) {
+        if (!(ok = wait(&bars->full[s], ph))) break;
         tc_fence_after();
-        const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
+        uint32_t a_lo = (uint32_t)da + s * (L::kStage >> 4), b_lo = (uint32_t)db + s * (L::kStage >> 4);
 #pragma unroll
         for (int kk = 0; kk < kBK / 16; ++kk) {
-          // K-major: 16 of a row's 64; MN-major: 16 of 64 rows, 64-wide column blocks 8 KB apart
-          const uint64_t da = p.a_mn ? smem_desc(sa + kk * 2048, 8192, 1024, kSwizzle128B)
-                                     : smem_desc(sa + kk * 32, 16, 1024, kSwizzle128B);
-          const uint64_t db = p.b_mn ? smem_desc(sb + kk * 2048, 8192, 1024, kSwizzle128B)
-                                     : smem_desc(sb + kk * 32, 16, 1024, kSwizzle128B);
-          mma_pair(d, da, db, p.idesc, i > i0 || kk > 0);
+          mma_pair(d, ((uint64_t)a_hi << 32) | a_lo, ((uint64_t)b_hi << 32) | b_lo, p.idesc, more);
+          a_lo += a_step;
+          b_lo += b_step;
+          more = 1;
         }
         commit_pair(&bars->empty[s]);
+        if (++s == L::kStages) { s = 0; ph ^= 1; }
       }
       if (ok) commit_pair(&bars->acc_full[buf]);
     }
-  } else if (warp == 3 && lane == 0 && p.res && p.res_tma) {
-    // ------------------------------------------------------------ residual tiles
-    int q = 0;  // chunks loaded per warp
-    bool ok = true;
-    for (int item = first; ok && item < p.items; item += step) {
-      int m0, n0, split, i0, i1;
-      tile_of(item, m0, n0, split, i0, i1);
-      for (int c = 0; ok && c < kChunks && n0 + c * kCols < p.N; ++c, ++q)
-        for (int w = 0; w < kEpiWarps; ++w) {  // rows past M load as zeros
-          const int row = m0 + (int)rank * 128 + w * 32;
-          if (!(ok = wait(&bars->res_free[w][q & 1], ((q >> 1) & 1) ^ 1))) break;
-          mbar_arrive_expect_tx(&bars->res_full[w][q & 1], kBuf);
-          tma_load_2d(sbase + L::OFF_RES + (w * 2 + (q & 1)) * kBuf, &map_res, n0 + c * kCols, row,
-                      &bars->res_full[w][q & 1]);
-        }
-    }
-    for (int j = q > 2 ? q - 2 : 0; ok && j < q; ++j)
-      for (int w = 0; ok && w < kEpiWarps; ++w) ok = wait(&bars->res_full[w][j & 1], (j >> 1) & 1);
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int w = warp & 3;
-    const uint32_t out_buf = sbase + L::OFF_OUT + w * 2 * kBuf, res_buf = sbase + L::OFF_RES + w * 2 * kBuf;
-    uint8_t* out_ptr = smem + L::OFF_OUT + w * 2 * kBuf;
-    float* s_bias = reinterpret_cast<float*>(smem + L::OFF_BIAS) + w * 64;
-    int t = 0, stores = 0, q = 0;
+    const int w = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes 32w.., columns half * BN/2..
+    const uint32_t sbuf = sbase + L::OFF_OUT + (warp - 4) * kBuf;
+    uint8_t* pbuf = smem + L::OFF_OUT + (warp - 4) * kBuf;
+    int t = 0;
     bool ok = true;
-    const bool same_way = !p.pre || p.pre_tma == p.out_tma;  // stores alternate between the buffers
-    const bool any_tma = p.out_tma || (p.pre && p.pre_tma);
-    // stages a buffer's rows and sends them out
-    auto send = [&](const float(&v)[kCols], const CUtensorMap* map, int tma, T* base, int64_t ld, int row, int n,
-                    int store_row) {
-      const int b = stores++ & 1;
-      if (any_tma) {  // the buffer's last store has read it
-        if (lane == 0) {
-          if (same_way) tma_store_wait_read<1>();
-          else tma_store_wait_read<0>();
-        }
-        __syncwarp();
-      }
-      write_row<T>(out_buf + b * kBuf, lane, v);
+    // sends the buffer's rows out, once every lane has written its own
+    auto send = [&](const CUtensorMap* map, int tma, T* base, int64_t ld, int row, int n, int store_row) {
       if (tma) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tma_store_2d(map, out_buf + b * kBuf, n, store_row);
+        if (lane == 0) tma_store_2d(map, sbuf, n, store_row);
       } else {
         __syncwarp();
-        copy_rows<T, true>(out_ptr + b * kBuf, base + (int64_t)row * ld + n, ld, min(32, p.M - row), p.N - n, lane);
-        __syncwarp();
+        copy_rows<T, true>(pbuf, base + (int64_t)row * ld + n, ld, min(32, p.M - row), p.N - n, lane);
       }
     };
+    auto buffer_free = [&]() {  // its last store, or the warp's own copies, have read it
+      if (lane == 0) tma_store_wait_read();
+      __syncwarp();
+    };
     for (int item = first; ok && item < p.items; item += step, ++t) {
-      int m0, n0, split, i0, i1;
-      tile_of(item, m0, n0, split, i0, i1);
+      const Item it = item_at<BN>(p, item);
       const int buf = t & 1;
-      const int row = m0 + (int)rank * 128 + w * 32;
+      const int row = it.m0 + (int)rank * 128 + w * 32;
+      const int n_first = it.n0 + half * (BN / 2);
+      const int n_end = row < p.M ? min(p.N, n_first + BN / 2) : 0;
+      const T* res = static_cast<const T*>(p.res) + (int64_t)row * p.ldr;
+      const bool res_vec = p.res && p.res_vec;
+      uint4 rv[8];
+      if (res_vec && n_first < n_end)
+        load_rows(res + n_first, p.ldr, p.M - row, p.N - n_first, lane, rv);
       ok = wait(&bars->acc_full[buf], (t >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t acc = tmem + buf * BN + ((uint32_t)(w * 32) << 16);
-      for (int c = 0; c < kChunks; ++c) {
-        const int n = n0 + c * kCols;
-        if (n >= p.N) break;
-        if (p.res && p.res_tma && row >= p.M) {  // its buffer turns over all the same
-          ok = wait(&bars->res_full[w][q & 1], (q >> 1) & 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+      const uint32_t acc = tmem + buf * BN + half * (BN / 2) + ((uint32_t)(w * 32) << 16);
+      for (int n = n_first; n < n_end; n += kCols) {
+        float v[kCols];
+#pragma unroll
+        for (int h = 0; h < kCols / 32; ++h)
+          tmem_ld32(acc + (n - n_first) + h * 32, *reinterpret_cast<float(*)[32]>(&v[h * 32]));
+        tmem_wait_ld();
+        if (p.bias) add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, p.N - n, v);
+        if (p.pre) {
+          buffer_free();
+          write_row<T>(sbuf, lane, v);
+          send(&map_pre, p.pre_tma, static_cast<T*>(p.pre), p.N, row, n, row);
+        }
+        activate<T>(v, p.act);
+        buffer_free();
+        if (p.res) {
+          if (res_vec) {
+            put_rows(sbuf, lane, rv);
+            if (n + kCols < n_end)
+              load_rows(res + n + kCols, p.ldr, p.M - row, p.N - n - kCols, lane, rv);
+          } else {
+            copy_rows<T, false>(pbuf, const_cast<T*>(res) + n, p.ldr, min(32, p.M - row), p.N - n, lane);
+          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->res_free[w][q & 1]);
+          add_row<T>(sbuf, lane, v);
         }
-        if (row < p.M) {
-          float v[kCols];
-          if (p.bias) {
-            __syncwarp();
-            for (int j = lane; j < kCols; j += 32)
-              s_bias[j] = n + j < p.N ? Elem<T>::load(static_cast<const T*>(p.bias) + n + j) : 0.f;
-          }
-#pragma unroll
-          for (int h = 0; h < kCols / 32; ++h)
-            tmem_ld32(acc + c * kCols + h * 32, *reinterpret_cast<float(*)[32]>(&v[h * 32]));
-          tmem_wait_ld();
-          if (p.bias) {
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < kCols; j += 4) {
-              const float4 bv = *reinterpret_cast<const float4*>(s_bias + j);
-              v[j] += bv.x; v[j + 1] += bv.y; v[j + 2] += bv.z; v[j + 3] += bv.w;
-            }
-          }
-          if (p.pre) send(v, &map_pre, p.pre_tma, static_cast<T*>(p.pre), p.N, row, n, row);
-          switch (p.act) {  // one loop per activation, so that the choice is made once per chunk
-            case MURM_ACT_NONE: break;
-            case MURM_ACT_RELU:
-#pragma unroll
-              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_RELU);
-              break;
-            case MURM_ACT_SILU:
-#pragma unroll
-              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_SILU);
-              break;
-            case MURM_ACT_GELU:
-#pragma unroll
-              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_GELU);
-              break;
-            default:
-#pragma unroll
-              for (int j = 0; j < kCols; ++j) v[j] = act_value<Out<T>::kFast>(v[j], MURM_ACT_GELU_TANH);
-          }
-          if (p.res) {
-            if (p.res_tma) {
-              const int b = q & 1;
-              ok = wait(&bars->res_full[w][b], (q >> 1) & 1);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              add_row<T>(res_buf + b * kBuf, lane, v);
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars->res_free[w][b]);
-            } else {
-              const T* res = static_cast<const T*>(p.res) + (int64_t)row * p.ldr + n;
-              copy_rows<T, false>(smem + L::OFF_RES + w * 2 * kBuf, const_cast<T*>(res), p.ldr, min(32, p.M - row),
-                                  p.N - n, lane);
-              __syncwarp();
-              add_row<T>(res_buf, lane, v);
-              __syncwarp();
-            }
-          }
-          send(v, &map_out, p.out_tma, static_cast<T*>(p.out), p.ldo, row, n, split * p.split_rows + row);
-        }
-        ++q;
+        write_row<T>(sbuf, lane, v);
+        send(&map_out, p.out_tma, static_cast<T*>(p.out), p.ldo, row, n, it.split * p.split_rows + row);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_remote(map_to_first(&bars->acc_free[buf]));
     }
-    if (lane == 0) tma_store_wait_read<0>();
+    if (lane == 0) tma_store_wait_read();
   }
   __syncwarp();
   tc_fence_before();
@@ -643,7 +640,7 @@ murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t
   constexpr int kCols = Out<T>::kCols;
   const CUtensorMapDataType op = g.dtype == MURM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapDataType ot = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(g.dtype);
-  CUtensorMap ma, mb, mo{}, mr{}, mp{};
+  CUtensorMap ma, mb, mo{}, mp{};
   CUresult r;
   if (g.a_mn) r = encode(&ma, op, 2, g.a.p, g.M, g.K, g.a.ld, g.a.planes, g.a.plane, 64, 64);
   else r = encode(&ma, op, 2, g.a.p, g.K, g.M, g.a.ld, g.a.planes, g.a.plane, 64, 128);
@@ -655,10 +652,9 @@ murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t
   p.ldo = ldo;
   p.out_tma = tma_rows(out, ldo, es);
   if (r == CUDA_SUCCESS && p.out_tma) r = encode(&mo, ot, es, out, out_cols, out_rows, ldo, 0, 0, kCols, 32);
-  if (p.res) {
-    p.res_tma = tma_rows(p.res, p.ldr, es);
-    if (r == CUDA_SUCCESS && p.res_tma) r = encode(&mr, ot, es, p.res, g.N, g.M, p.ldr, 0, 0, kCols, 32);
-  }
+  const int per = 16 / (int)es;
+  p.res_vec = p.res && tma_rows(p.res, p.ldr, es) && g.N % per == 0;
+  p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && g.N % per == 0;
   if (p.pre) {
     p.pre_tma = tma_rows(p.pre, g.N, es);
     if (r == CUDA_SUCCESS && p.pre_tma) r = encode(&mp, ot, es, p.pre, g.N, g.M, g.N, 0, 0, kCols, 32);
@@ -672,7 +668,7 @@ murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t
   const int grid = 2 * (items < kPairs ? items : kPairs);
   if (cudaError_t e = smem_opt_in(k_gemm_tc<T, BN>, Tile<BN>::kSmem))
     return report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
-  launch("linear_gemm", k_gemm_tc<T, BN>, dim3(grid), kThreads, Tile<BN>::kSmem, st, ma, mb, mo, mr, mp, p);
+  launch("linear_gemm", k_gemm_tc<T, BN>, dim3(grid), kThreads, Tile<BN>::kSmem, st, ma, mb, mo, mp, p);
   return MURM_OK;
 }
 
@@ -681,6 +677,7 @@ murm_status run(const Gemm& g, const Config& c, void* workspace, cudaStream_t st
   Args p{};
   p.M = g.M; p.N = g.N;
   p.kblocks = c.kblocks; p.iters = c.iters; p.total = c.total; p.splits = c.splits;
+  p.tiles_m = c.tiles_m;
   p.tiles_n = c.tiles_n;
   p.tiles = c.tiles_m * c.tiles_n;
   p.items = p.tiles * c.splits;
