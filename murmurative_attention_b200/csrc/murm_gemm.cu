@@ -7,10 +7,10 @@
 // k_gemm_tc: a pair of CTAs (cta_group::2) per 256 x BN tile, each holding 128 rows of A, half the
 // rows of B and a 128 x BN fp32 accumulator in TMEM (two accumulators: a tile's epilogue runs under
 // the next tile's products). Persistent over the tiles. Warp 0 loads the operands by TMA into a
-// ring of 64-deep stages, warp 1 of the first CTA issues the MMAs of both, warps 4-11 run the
-// epilogue, each on 32 rows and half the columns: TMEM -> registers -> bias, activation, residual ->
-// 128-byte swizzled rows in shared memory -> TMA store (or plain stores where the result's rows are
-// not 16-byte aligned).
+// ring of 64-deep stages, warp 1 of the first CTA issues the MMAs of both, warps 4-19 run the
+// epilogue, each on 32 rows and a quarter of the columns: TMEM -> registers -> bias, activation,
+// residual -> 64-byte swizzled rows in shared memory -> TMA store (or plain stores where the
+// result's rows are not 16-byte aligned).
 //
 // fp32 operands are three bf16 planes; the products of planes (i, j) with i + j <= 2 carry them to
 // 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K
@@ -36,9 +36,9 @@ constexpr int kSms = 148;
 constexpr int kPairs = kSms / 2;     // CTA pairs resident at once
 constexpr int kBK = 64;              // depth of a stage: one 128-byte swizzled row
 constexpr uint32_t kABytes = 128 * kBK * 2;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;        // 4 row groups (TMEM lanes) x 4 column groups
 constexpr int kThreads = 128 + 32 * kEpiWarps;
-constexpr uint32_t kBuf = 32 * 128;  // one epilogue warp's 32 rows of 128 bytes
+constexpr uint32_t kBuf = 32 * 64;   // one epilogue warp's 32 rows of 64 bytes
 
 template <int BN> struct Tile {
   static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
@@ -148,13 +148,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
 // ---------------------------------------------------------------------------
 // epilogue pieces
 // ---------------------------------------------------------------------------
-template <typename T> struct Out {  // 16-bit results: 64 columns in a 128-byte row
-  static constexpr int kCols = 64;
-  static constexpr bool kFast = true;
-};
-template <> struct Out<float> {
-  static constexpr int kCols = 32;
-  static constexpr bool kFast = false;
+template <typename T> struct Out {  // an epilogue step: 64 bytes of a row
+  static constexpr int kCols = 64 / sizeof(T);
+  static constexpr bool kFast = sizeof(T) == 2;
 };
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
@@ -181,11 +177,14 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// A lane's 128-byte row of a swizzled buffer: chunk j of 16 bytes sits at j ^ (row mod 8).
+// Chunk j of 16 bytes of row r in a buffer of 64-byte rows (the tensor engine's 64-byte swizzle).
+__device__ __forceinline__ uint32_t chunk_at(int r, int j) { return r * 64 + ((j ^ ((r >> 1) & 3)) << 4); }
+
+// A lane's own row.
 template <typename T>
 __device__ __forceinline__ void write_row(uint32_t buf, int lane, const float (&v)[Out<T>::kCols]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     uint4 u;
     if constexpr (sizeof(T) == 2) {
       u.x = pack2(v[8 * j], v[8 * j + 1], (const T*)nullptr);
@@ -196,72 +195,71 @@ __device__ __forceinline__ void write_row(uint32_t buf, int lane, const float (&
       u = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
                      __float_as_uint(v[4 * j + 3]));
     }
-    sts128(buf + lane * 128 + ((j ^ (lane & 7)) << 4), u);
+    sts128(buf + chunk_at(lane, j), u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add16(const uint4& u, float* v) {  // v += the elements of 16 bytes
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = unpack2(w[i], (const T*)nullptr);
+      v[2 * i] += f.x;
+      v[2 * i + 1] += f.y;
+    } else {
+      v[i] += __uint_as_float(w[i]);
+    }
   }
 }
 template <typename T>
 __device__ __forceinline__ void add_row(uint32_t buf, int lane, float (&v)[Out<T>::kCols]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint4 u = lds128(buf + lane * 128 + ((j ^ (lane & 7)) << 4));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        const float2 f = unpack2(w[i], (const T*)nullptr);
-        v[8 * j + 2 * i] += f.x;
-        v[8 * j + 2 * i + 1] += f.y;
-      } else {
-        v[4 * j + i] += __uint_as_float(w[i]);
-      }
-    }
-  }
+  for (int j = 0; j < 4; ++j) add16<T>(lds128(buf + chunk_at(lane, j)), v + j * (16 / sizeof(T)));
 }
-// A warp's 32 rows of a buffer in global memory, eight lanes to a row: coalesced 16-byte accesses.
+// A warp's 32 rows of a buffer in global memory, four lanes to a row: coalesced 16-byte accesses.
 template <typename T>
-__device__ __forceinline__ void load_rows(const T* g, int64_t ld, int rows, int cols, int lane, uint4 (&v)[8]) {
-  const int c = (lane & 7) * (16 / (int)sizeof(T));
+__device__ __forceinline__ void load_rows(const T* g, int64_t ld, int rows, int cols, int lane, uint4 (&v)[4]) {
+  const int c = (lane & 3) * (16 / (int)sizeof(T));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
     v[i] = make_uint4(0, 0, 0, 0);
     if (r < rows && c < cols) v[i] = __ldg(reinterpret_cast<const uint4*>(g + r * ld + c));
   }
 }
-__device__ __forceinline__ void put_rows(uint32_t buf, int lane, const uint4 (&v)[8]) {
+__device__ __forceinline__ void put_rows(uint32_t buf, int lane, const uint4 (&v)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
-    sts128(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4), v[i]);
-  }
+  for (int i = 0; i < 4; ++i) sts128(buf + chunk_at(i * 8 + (lane >> 2), lane & 3), v[i]);
 }
 // The same rows where 16-byte accesses are not aligned: element by element, columns side by side.
 template <typename T, bool STORE>
 __device__ __forceinline__ void copy_rows(uint8_t* buf, T* g, int64_t ld, int rows, int cols, int lane) {
-  for (int r = 0; r < rows; ++r)
-#pragma unroll
-    for (int c = lane; c < Out<T>::kCols; c += 32) {
-      T* s = reinterpret_cast<T*>(buf + r * 128 + ((((c * (int)sizeof(T)) >> 4) ^ (r & 7)) << 4) +
-                                  ((c * (int)sizeof(T)) & 15));
-      if (c < cols) {
-        if (STORE) g[r * ld + c] = *s;
-        else *s = g[r * ld + c];
-      }
-    }
+  constexpr int kCols = Out<T>::kCols, kRows = 32 / kCols;  // columns of a row, rows side by side
+  const int c = lane % kCols;
+  if (c >= cols) return;
+  for (int r = lane / kCols; r < rows; r += kRows) {
+    T* s = reinterpret_cast<T*>(buf + chunk_at(r, (c * (int)sizeof(T)) >> 4) + ((c * (int)sizeof(T)) & 15));
+    if (STORE) g[r * ld + c] = *s;
+    else *s = g[r * ld + c];
+  }
 }
-// v += the bias of a chunk's columns: the same address in every lane, from L1.
+// The bias of a step's columns: the same address in every lane, from L1. With `vec`, b holds it
+// (loaded early, while the accumulator is on its way).
 template <typename T>
-__device__ __forceinline__ void add_bias(const T* bias, int vec, int cols, float (&v)[Out<T>::kCols]) {
-  constexpr int kPer = 16 / sizeof(T);
+__device__ __forceinline__ void load_bias(const T* bias, int cols, uint4 (&b)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    b[j] = make_uint4(0, 0, 0, 0);
+    if (j * (16 / (int)sizeof(T)) < cols) b[j] = __ldg(reinterpret_cast<const uint4*>(bias) + j);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add_bias(const T* bias, int vec, const uint4 (&b)[4], int cols,
+                                         float (&v)[Out<T>::kCols]) {
   if (vec) {
 #pragma unroll
-    for (int j = 0; j < Out<T>::kCols / kPer; ++j) {
-      if (j * kPer >= cols) break;
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(bias) + j);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) v[j * kPer + i] += Elem<T>::load(e + i);
-    }
+    for (int j = 0; j < 4; ++j) add16<T>(b[j], v + j * (16 / sizeof(T)));
   } else {
 #pragma unroll
     for (int j = 0; j < Out<T>::kCols; ++j)
@@ -427,7 +425,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int w = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes 32w.., columns half * BN/2..
+    const int w = warp & 3, quarter = (warp - 4) >> 2;  // TMEM lanes 32w.., columns quarter * BN/4..
     const uint32_t sbuf = sbase + L::OFF_OUT + (warp - 4) * kBuf;
     uint8_t* pbuf = smem + L::OFF_OUT + (warp - 4) * kBuf;
     int t = 0;
@@ -451,25 +449,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item it = item_at<BN>(p, item);
       const int buf = t & 1;
       const int row = it.m0 + (int)rank * 128 + w * 32;
-      const int n_first = it.n0 + half * (BN / 2);
-      const int n_end = row < p.M ? min(p.N, n_first + BN / 2) : 0;
+      const int n_first = it.n0 + quarter * (BN / 4);
+      const int n_end = row < p.M ? min(p.N, n_first + BN / 4) : 0;
       const T* res = static_cast<const T*>(p.res) + (int64_t)row * p.ldr;
       const bool res_vec = p.res && p.res_vec;
-      uint4 rv[8];
+      uint4 rv[4], bv[4];
       if (res_vec && n_first < n_end)
         load_rows(res + n_first, p.ldr, p.M - row, p.N - n_first, lane, rv);
+      if (p.bias_vec && n_first < n_end) load_bias(static_cast<const T*>(p.bias) + n_first, p.N - n_first, bv);
       ok = wait(&bars->acc_full[buf], (t >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t acc = tmem + buf * BN + half * (BN / 2) + ((uint32_t)(w * 32) << 16);
+      const uint32_t acc = tmem + buf * BN + quarter * (BN / 4) + ((uint32_t)(w * 32) << 16);
       for (int n = n_first; n < n_end; n += kCols) {
         float v[kCols];
-#pragma unroll
-        for (int h = 0; h < kCols / 32; ++h)
-          tmem_ld32(acc + (n - n_first) + h * 32, *reinterpret_cast<float(*)[32]>(&v[h * 32]));
+        if constexpr (kCols == 32) tmem_ld32(acc + (n - n_first), v);
+        else tmem_ld16(acc + (n - n_first), v);
         tmem_wait_ld();
-        if (p.bias) add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, p.N - n, v);
+        if (p.bias) {
+          add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, bv, p.N - n, v);
+          if (p.bias_vec && n + kCols < n_end)
+            load_bias(static_cast<const T*>(p.bias) + n + kCols, p.N - n - kCols, bv);
+        }
         if (p.pre) {
           buffer_free();
           write_row<T>(sbuf, lane, v);
@@ -611,6 +613,8 @@ Config choose(const Gemm& g) {
   return best;
 }
 
+// Operands: three dimensions (the planes) and 128-byte swizzled rows; results (planes = 0): two
+// dimensions and the epilogue's 64-byte rows.
 CUresult encode(CUtensorMap* map, CUtensorMapDataType type, size_t es, const void* p, int64_t cols, int64_t rows,
                 int64_t ld, int planes, int64_t plane, int box_cols, int box_rows) {
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
@@ -618,7 +622,8 @@ CUresult encode(CUtensorMap* map, CUtensorMapDataType type, size_t es, const voi
   cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
   cuuint32_t unit[3] = {1, 1, 1};
   return tc_tensor_map_encoder()(map, type, planes ? 3 : 2, const_cast<void*>(p), dims, strides, box, unit,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 planes ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 

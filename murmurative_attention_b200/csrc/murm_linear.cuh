@@ -54,47 +54,62 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // FAST: for results rounded to 16 bits, with the hardware's exp2 and reciprocal (relative errors
 // near 2^-22); else CUDA's accurate functions.
-template <bool FAST>
-__device__ __forceinline__ float exp_(float x) {
-  if (!FAST) return expf(x);
+__device__ __forceinline__ float ex2_(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * kLog2e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-template <bool FAST>
 __device__ __forceinline__ float rcp_(float x) {
-  if (!FAST) return 1.f / x;
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// 1 / (1 + exp(-(a + b x^2) x)): the sigmoid (a = 1, b = 0) and gelu's tanh form
 template <bool FAST>
-__device__ __forceinline__ float sigmoid_(float x) { return rcp_<FAST>(1.f + exp_<FAST>(-x)); }
+__device__ __forceinline__ float sigmoid_(float x, float a, float b) {
+  if (FAST) return rcp_(1.f + ex2_(x * fmaf(x * x, -b * kLog2e, -a * kLog2e)));
+  return 1.f / (1.f + expf(-x * (a + b * (x * x))));
+}
+template <bool FAST>
+__device__ __forceinline__ float silu_sigmoid(float x) {
+  if (FAST) return rcp_(1.f + ex2_(-kLog2e * x));
+  return 1.f / (1.f + expf(-x));
+}
+constexpr float kTanhA = 2.f * kSqrt2OverPi, kTanhB = 2.f * kSqrt2OverPi * 0.044715f;
 
-// The standard normal distribution function. FAST: 0.5 erfc(|z| / sqrt 2) by formula 7.1.26 of
-// Abramowitz and Stegun (absolute error of erf at most 1.5e-7), with the argument's 1/sqrt 2 and
-// the result's 1/2 folded into the coefficients.
-template <bool FAST>
-__device__ __forceinline__ float normal_cdf(float z) {
-  if (!FAST) return 0.5f * (1.f + erff(z * kSqrtHalf));
-  const float a = fabsf(z);
-  const float t = rcp_<true>(fmaf(0.3275911f * kSqrtHalf, a, 1.f));
+// 0.5 erfc(a / sqrt 2) for a >= 0, the standard normal distribution's upper tail, and exp(-a^2/2)
+// beside it: formula 7.1.26 of Abramowitz and Stegun (absolute error of erf at most 1.5e-7), with
+// the argument's 1/sqrt 2 and the result's 1/2 folded into the coefficients.
+__device__ __forceinline__ float normal_tail(float a, float& e) {
+  const float t = rcp_(fmaf(0.3275911f * kSqrtHalf, a, 1.f));
   float q = fmaf(t, 0.5f * 1.061405429f, -0.5f * 1.453152027f);
   q = fmaf(q, t, 0.5f * 1.421413741f);
   q = fmaf(q, t, -0.5f * 0.284496736f);
   q = fmaf(q, t, 0.5f * 0.254829592f);
-  q *= t * exp_<true>(-0.5f * z * z);
-  return z < 0.f ? q : 1.f - q;  // NaN: q is NaN
+  e = ex2_(-0.5f * kLog2e * a * a);
+  return q * t * e;
+}
+// max(z, 0), NaN for NaN
+__device__ __forceinline__ float relu_(float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+  return r;
 }
 
 template <bool FAST>
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
-    case MURM_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps NaN
-    case MURM_ACT_SILU: return z * sigmoid_<FAST>(z);
-    case MURM_ACT_GELU: return z * normal_cdf<FAST>(z);
+    case MURM_ACT_RELU: return relu_(z);
+    case MURM_ACT_SILU: return z * silu_sigmoid<FAST>(z);
+    case MURM_ACT_GELU:
+      if (FAST) {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|); past 30 the second term is 0
+        float e;
+        const float a = fminf(fabsf(z), 30.f);
+        return fmaf(-a, normal_tail(a, e), relu_(z));
+      }
+      return 0.5f * z * (1.f + erff(z * kSqrtHalf));
     case MURM_ACT_GELU_TANH:  // 0.5 (1 + tanh u) = sigmoid(2u)
-      return z * sigmoid_<FAST>(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
+      return z * sigmoid_<FAST>(z, kTanhA, kTanhB);
   }
   return z;
 }
@@ -104,13 +119,19 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case MURM_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case MURM_ACT_SILU: {
-      const float s = sigmoid_<FAST>(z);
+      const float s = silu_sigmoid<FAST>(z);
       return s * (1.f + z * (1.f - s));
     }
-    case MURM_ACT_GELU: return normal_cdf<FAST>(z) + z * kInvSqrt2Pi * exp_<FAST>(-0.5f * z * z);
+    case MURM_ACT_GELU:
+      if (FAST) {
+        float e;
+        const float q = normal_tail(fabsf(z), e);
+        return fmaf(z * kInvSqrt2Pi, e, z < 0.f ? q : 1.f - q);
+      }
+      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expf(-0.5f * z * z);
     case MURM_ACT_GELU_TANH: {
-      const float s = sigmoid_<FAST>(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
-      return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * 0.044715f * z * z);
+      const float s = sigmoid_<FAST>(z, kTanhA, kTanhB);
+      return s + z * s * (1.f - s) * (kTanhA + 3.f * kTanhB * z * z);
     }
   }
   return 1.f;
