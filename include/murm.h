@@ -424,11 +424,11 @@ MURM_API size_t murm_norm_rope_workspace(void);
  * with unit inner stride and the given row strides (any element alignment),
  * residual and out [rows, out_features] likewise, bias [out_features]. Sums
  * are in fp32 (fp32 inputs: exact three-term bf16 splits, fp32 accuracy).
- * preact, when not NULL, receives z in `dtype` ([rows, out_features]
+ * slope, when not NULL, receives act'(z) in `dtype` ([rows, out_features]
  * contiguous) for the backward; it is needed there unless the activation is
- * MURM_ACT_NONE.
+ * MURM_ACT_NONE, which writes none.
  *
- * Backward: dz = grad_out * act'(z), rounded once to `dtype` where it becomes a
+ * Backward: dz = grad_out * slope, rounded once to `dtype` where it becomes a
  * matrix operand; grad_x = dz W, grad_weight = dz^T x, grad_bias = column sums of
  * the unrounded dz (fixed order). Each output may be NULL. rows may be 0. */
 typedef enum murm_activation {
@@ -445,7 +445,7 @@ typedef struct murm_linear_args {
   const void* bias;                           /* or NULL */
   const void* residual; int64_t r_stride;     /* or NULL */
   void* out; int64_t out_stride;
-  void* preact;                               /* or NULL */
+  void* slope;                                /* or NULL */
   void* workspace; size_t workspace_bytes;
 } murm_linear_args;
 
@@ -454,7 +454,7 @@ typedef struct murm_linear_bwd_args {
   int32_t in_features, out_features, dtype, activation;
   const void* x; int64_t x_stride;
   const void* weight; int64_t w_stride;
-  const void* preact;                         /* as the forward wrote it */
+  const void* slope;                          /* as the forward wrote it */
   const void* grad_out; int64_t go_stride;
   void* grad_x; int64_t gx_stride;            /* each gradient: or NULL */
   void* grad_weight; int64_t gw_stride;

@@ -239,7 +239,7 @@ class LinearArgs(ctypes.Structure):
         ("bias", ctypes.c_void_p),
         ("residual", ctypes.c_void_p), ("r_stride", ctypes.c_int64),
         ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
-        ("preact", ctypes.c_void_p),
+        ("slope", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
@@ -250,7 +250,7 @@ class LinearBwdArgs(ctypes.Structure):
         ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
         ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
         ("weight", ctypes.c_void_p), ("w_stride", ctypes.c_int64),
-        ("preact", ctypes.c_void_p),
+        ("slope", ctypes.c_void_p),
         ("grad_out", ctypes.c_void_p), ("go_stride", ctypes.c_int64),
         ("grad_x", ctypes.c_void_p), ("gx_stride", ctypes.c_int64),
         ("grad_weight", ctypes.c_void_p), ("gw_stride", ctypes.c_int64),

@@ -69,7 +69,7 @@ struct Args {
   int act;
   const void* res; int64_t ldr; int res_vec;
   void* out; int64_t ldo; int out_tma;
-  void* pre; int pre_tma;
+  void* slope; int slope_tma;
   int split_rows;  // rows of one split's partial result
 };
 
@@ -180,23 +180,19 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 // Chunk j of 16 bytes of row r in a buffer of 64-byte rows (the tensor engine's 64-byte swizzle).
 __device__ __forceinline__ uint32_t chunk_at(int r, int j) { return r * 64 + ((j ^ ((r >> 1) & 3)) << 4); }
 
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* v) {  // 16 bytes of elements
+  if constexpr (sizeof(T) == 2)
+    return make_uint4(pack2(v[0], v[1], (const T*)nullptr), pack2(v[2], v[3], (const T*)nullptr),
+                      pack2(v[4], v[5], (const T*)nullptr), pack2(v[6], v[7], (const T*)nullptr));
+  else
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
 // A lane's own row.
 template <typename T>
 __device__ __forceinline__ void write_row(uint32_t buf, int lane, const float (&v)[Out<T>::kCols]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 u;
-    if constexpr (sizeof(T) == 2) {
-      u.x = pack2(v[8 * j], v[8 * j + 1], (const T*)nullptr);
-      u.y = pack2(v[8 * j + 2], v[8 * j + 3], (const T*)nullptr);
-      u.z = pack2(v[8 * j + 4], v[8 * j + 5], (const T*)nullptr);
-      u.w = pack2(v[8 * j + 6], v[8 * j + 7], (const T*)nullptr);
-    } else {
-      u = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
-                     __float_as_uint(v[4 * j + 3]));
-    }
-    sts128(buf + chunk_at(lane, j), u);
-  }
+  for (int j = 0; j < 4; ++j) sts128(buf + chunk_at(lane, j), pack16<T>(v + j * (16 / sizeof(T))));
 }
 template <typename T>
 __device__ __forceinline__ void add16(const uint4& u, float* v) {  // v += the elements of 16 bytes
@@ -266,26 +262,26 @@ __device__ __forceinline__ void add_bias(const T* bias, int vec, const uint4 (&b
       if (j < cols) v[j] += Elem<T>::load(bias + j);
   }
 }
-template <typename T>
-__device__ __forceinline__ void activate(float (&v)[Out<T>::kCols], int act) {
-  constexpr bool F = Out<T>::kFast;
+// v = act(v); SLOPE: the slopes go to the lane's row of the buffer, 16 bytes at a time.
+template <typename T, bool SLOPE, int ACT>
+__device__ __forceinline__ void activate_as(float (&v)[Out<T>::kCols], uint32_t buf, int lane) {
+  constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float d[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[j * kPer + i] = act_value<Out<T>::kFast>(v[j * kPer + i], ACT, d[i]);
+    if (SLOPE) sts128(buf + chunk_at(lane, j), pack16<T>(d));
+  }
+}
+template <typename T, bool SLOPE>
+__device__ __forceinline__ void activate(float (&v)[Out<T>::kCols], int act, uint32_t buf, int lane) {
   switch (act) {  // one loop per activation: the choice is made once
     case MURM_ACT_NONE: break;
-    case MURM_ACT_RELU:
-#pragma unroll
-      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_RELU);
-      break;
-    case MURM_ACT_SILU:
-#pragma unroll
-      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_SILU);
-      break;
-    case MURM_ACT_GELU:
-#pragma unroll
-      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_GELU);
-      break;
-    default:
-#pragma unroll
-      for (int j = 0; j < Out<T>::kCols; ++j) v[j] = act_value<F>(v[j], MURM_ACT_GELU_TANH);
+    case MURM_ACT_RELU: activate_as<T, SLOPE, MURM_ACT_RELU>(v, buf, lane); break;
+    case MURM_ACT_SILU: activate_as<T, SLOPE, MURM_ACT_SILU>(v, buf, lane); break;
+    case MURM_ACT_GELU: activate_as<T, SLOPE, MURM_ACT_GELU>(v, buf, lane); break;
+    default: activate_as<T, SLOPE, MURM_ACT_GELU_TANH>(v, buf, lane);
   }
 }
 
@@ -316,7 +312,7 @@ __device__ __forceinline__ Item item_at(const Args& p, int item) {
 template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_pre,
+              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_slope,
               const __grid_constant__ Args p) {
   using L = Tile<BN>;
   constexpr int kCols = Out<T>::kCols;
@@ -472,12 +468,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (p.bias_vec && n + kCols < n_end)
             load_bias(static_cast<const T*>(p.bias) + n + kCols, p.N - n - kCols, bv);
         }
-        if (p.pre) {
+        if (p.slope) {
           buffer_free();
-          write_row<T>(sbuf, lane, v);
-          send(&map_pre, p.pre_tma, static_cast<T*>(p.pre), p.N, row, n, row);
+          activate<T, true>(v, p.act, sbuf, lane);
+          send(&map_slope, p.slope_tma, static_cast<T*>(p.slope), p.N, row, n, row);
+        } else {
+          activate<T, false>(v, p.act, sbuf, lane);
         }
-        activate<T>(v, p.act);
         buffer_free();
         if (p.res) {
           if (res_vec) {
@@ -526,8 +523,8 @@ __global__ void __launch_bounds__(256)
   for (int j = 0; j < 4; ++j) {
     if (n + j >= p.N) break;
     if (p.bias) z[j] += Elem<T>::load(static_cast<const T*>(p.bias) + n + j);
-    if (p.pre) Elem<T>::store(static_cast<T*>(p.pre) + m * p.N + n + j, z[j]);
-    float y = act_value<Out<T>::kFast>(z[j], p.act);
+    float slope, y = act_value<Out<T>::kFast>(z[j], p.act, slope);
+    if (p.slope) Elem<T>::store(static_cast<T*>(p.slope) + m * p.N + n + j, slope);
     if (p.res) y += Elem<T>::load(static_cast<const T*>(p.res) + m * p.ldr + n + j);
     Elem<T>::store(static_cast<T*>(p.out) + m * p.ldo + n + j, y);
   }
@@ -587,8 +584,13 @@ struct Config {
   int bn, splits, iters, total, kblocks, tiles_m, tiles_n;
 };
 
-// Tile width and K splits by estimated time, in units of one stage of a 256-wide tile (512 clocks):
-// rounds of the pairs over the items times the item's stages plus its fill and drain.
+// Tile width and K splits by estimated time, in microseconds measured on B200:
+// - a 64-deep stage takes 0.35 of a 256-wide tile (its 64 KB per CTA pair are about what L2 delivers
+//   to two SMs in that time, which is also the MMAs' own) and 0.31 of a 128-wide one, bound by the
+//   rows of A it loads all the same; 15 % more where A is read MN-major. So 128 pays only where it
+//   leaves fewer rounds: 512 x 1024 x 1024: 9.5 us at 128, 10.2 at 256; 8192 x 1024 x 1024: 27.5 and 18.1.
+// - a split costs a second launch, and its fp32 sums about 4.8 MB per us:
+//   1024 x 1024 x 8192 (dW): 50 us in one part, 24 in four, 28 in eight.
 Config choose(const Gemm& g) {
   Config best{};
   double best_t = 0;
@@ -597,13 +599,14 @@ Config choose(const Gemm& g) {
   for (int bn : {256, 128}) {
     const int tm = (g.M + 255) / 256, tn = (g.N + bn - 1) / bn;
     const int64_t tiles = (int64_t)tm * tn;
-    for (int splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (total / splits < 4 || tiles * splits > 2 * kPairs)) break;
+    const double stage = (bn == 256 ? 0.35 : 0.31) * (g.a_mn ? 1.15 : 1.0);
+    for (int splits = 1; splits <= 16; ++splits) {
+      if (splits > 1 && (total / splits < 2 || tiles * splits > 2 * kPairs)) break;
       const int iters = (total + splits - 1) / splits;
       const int used = (total + iters - 1) / iters;
       const int64_t rounds = (tiles * used + kPairs - 1) / kPairs;
-      double t = rounds * (iters * (bn / 256.0)) + 6;
-      if (used > 1) t += 8 + (double)g.M * g.N * 4 * (used + 1) / 1.5e6;
+      double t = rounds * iters * stage;
+      if (used > 1) t += 4.0 + (double)tiles * 256 * bn * 4 * used / 4.8e6;
       if (best_t == 0 || t < best_t) {
         best_t = t;
         best = Config{bn, used, iters, total, kblocks, tm, tn};
@@ -645,7 +648,7 @@ murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t
   constexpr int kCols = Out<T>::kCols;
   const CUtensorMapDataType op = g.dtype == MURM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapDataType ot = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(g.dtype);
-  CUtensorMap ma, mb, mo{}, mp{};
+  CUtensorMap ma, mb, mo{}, ms{};
   CUresult r;
   if (g.a_mn) r = encode(&ma, op, 2, g.a.p, g.M, g.K, g.a.ld, g.a.planes, g.a.plane, 64, 64);
   else r = encode(&ma, op, 2, g.a.p, g.K, g.M, g.a.ld, g.a.planes, g.a.plane, 64, 128);
@@ -660,9 +663,9 @@ murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t
   const int per = 16 / (int)es;
   p.res_vec = p.res && tma_rows(p.res, p.ldr, es) && g.N % per == 0;
   p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && g.N % per == 0;
-  if (p.pre) {
-    p.pre_tma = tma_rows(p.pre, g.N, es);
-    if (r == CUDA_SUCCESS && p.pre_tma) r = encode(&mp, ot, es, p.pre, g.N, g.M, g.N, 0, 0, kCols, 32);
+  if (p.slope) {
+    p.slope_tma = tma_rows(p.slope, g.N, es);
+    if (r == CUDA_SUCCESS && p.slope_tma) r = encode(&ms, ot, es, p.slope, g.N, g.M, g.N, 0, 0, kCols, 32);
   }
   if (r != CUDA_SUCCESS) {
     char msg[96];
@@ -673,7 +676,7 @@ murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t
   const int grid = 2 * (items < kPairs ? items : kPairs);
   if (cudaError_t e = smem_opt_in(k_gemm_tc<T, BN>, Tile<BN>::kSmem))
     return report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
-  launch("linear_gemm", k_gemm_tc<T, BN>, dim3(grid), kThreads, Tile<BN>::kSmem, st, ma, mb, mo, mp, p);
+  launch("linear_gemm", k_gemm_tc<T, BN>, dim3(grid), kThreads, Tile<BN>::kSmem, st, ma, mb, mo, ms, p);
   return MURM_OK;
 }
 
@@ -691,7 +694,7 @@ murm_status run(const Gemm& g, const Config& c, void* workspace, cudaStream_t st
   p.fp32 = g.a.planes == 3;
   p.bias = g.bias; p.act = g.act;
   p.res = g.res; p.ldr = g.ldr;
-  p.pre = g.preact;
+  p.slope = g.slope;
   murm_status s;
   if (c.splits == 1) {
     s = c.bn == 256 ? launch_tc<T, 256>(g, c, p, g.out, g.ldo, g.M, g.N, st)
@@ -699,7 +702,7 @@ murm_status run(const Gemm& g, const Config& c, void* workspace, cudaStream_t st
   } else {
     Args q = p;  // partial sums alone
     q.bias = q.res = nullptr;
-    q.pre = nullptr;
+    q.slope = nullptr;
     q.act = MURM_ACT_NONE;
     const int rows = c.tiles_m * 256, cols = c.tiles_n * c.bn;
     q.M = rows;

@@ -1,8 +1,8 @@
 // murm_linear.cu — the linear layer's C ABI and its elementwise backward.
 //
 // Forward: one matrix product with bias, activation and residual in its epilogue (murm_gemm.cu).
-// Backward: dz = dy * act'(z) and db = column sums of dz in one pass over dy and z, then
-// dx = dz W and dW = dz^T x. Without an activation dz is dy itself and the pass only sums it.
+// Backward: dz = dy * act'(z), from the slopes the forward saved, and db = column sums of dz in one
+// pass over both, then dx = dz W and dW = dz^T x. Without an activation dz is dy itself and the pass only sums it.
 #include <cstdarg>
 #include <cstdio>
 
@@ -24,11 +24,10 @@ murm_status bad(murm_status s, const char* fmt, ...) {
 }
 
 // ---------------------------------------------------------------------------
-// dz = dy * act'(z), db
+// dz = dy * slope, db
 // ---------------------------------------------------------------------------
-constexpr int kDzCols = 32;     // column groups (of V columns) per block, a warp wide
-constexpr int kDzRows = 8;      // rows a block has in flight
-constexpr int kDzChunks = 128;  // most row chunks, each with one partial of db
+constexpr int kDzThreads = 256;
+constexpr int kDzChunks = 512;  // most row chunks, each with one partial of db
 
 template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T e[V]; };
 
@@ -55,47 +54,72 @@ __device__ __forceinline__ void store_operand(const Operand& o, int64_t at, cons
   }
 }
 
-// Block (x, y): V * 32 columns, a chunk of rows; 8 warps take the chunk's rows in turn. db sums dz
-// unrounded, in fp32: a thread's rows in order, then the block's 8 warps in order, then (k_col_sum)
-// the chunks in order.
-template <typename T, int V>
-__global__ void __launch_bounds__(kDzCols * kDzRows)
-    k_dz(const T* dy, int64_t ldy, const T* z, int M, int N, int act, int chunk,
-         Operand dz, float* part) {
-  __shared__ float s[kDzRows][kDzCols * V + 1];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int n = (blockIdx.x * kDzCols + tx) * V;
-  const int m0 = blockIdx.y * chunk, m1 = min(M, m0 + chunk);
+// Block (x, y): `cols` threads side by side (a power of two, as many as a row has groups of V
+// columns, up to the block), the others on further rows; a chunk of rows. db sums dz unrounded, in
+// fp32: a thread's rows in order, then the block's row groups in order, then (k_col_sum) the chunks.
+//
+// Bound by memory: dy and the slopes read once, dz written once; 32768 x 4096 bf16 takes 129 us
+// (6.3 TB/s). A row's columns go to neighbouring threads and a thread issues kDzDepth rows' loads
+// together; with a bounds check at each of them they went out one by one (180 us), so full batches
+// run without and single rows follow.
+constexpr int kDzDepth = 4;
+
+template <typename T, int V, bool SLOPE>
+__global__ void __launch_bounds__(kDzThreads, 3)
+    k_dz(const T* dy, int64_t ldy, const T* slope, int M, int N, int cols, int chunk, Operand dz, float* part) {
+  __shared__ float s[kDzThreads * V];  // [row group][column]
+  const int tx = threadIdx.x & (cols - 1), ty = threadIdx.x / cols, rows = kDzThreads / cols;
+  const int n = (blockIdx.x * cols + tx) * V;
+  const int m1 = (int)min((int64_t)M, (int64_t)(blockIdx.y + 1) * chunk);
+  constexpr int kDepth = SLOPE ? kDzDepth : 2 * kDzDepth;
+  using P = Pack<T, V>;
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  auto row = [&](int r, const P& g, const P& sl) {
+    float d[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      d[e] = Elem<T>::load(g.e + e);
+      if (SLOPE) d[e] *= Elem<T>::load(sl.e + e);
+      acc[e] += d[e];
+    }
+    if (SLOPE && dz.p) store_operand<T, V>(dz, (int64_t)r * dz.ld + n, d);
+  };
   if (n < N) {  // V divides N
-    using P = Pack<T, V>;
-#pragma unroll 4
-    for (int m = m0 + ty; m < m1; m += kDzRows) {
-      const P g = *reinterpret_cast<const P*>(dy + (int64_t)m * ldy + n);
-      float d[V];
+    int m = blockIdx.y * chunk + ty;
+    const T* pg = dy + (int64_t)m * ldy + n;
+    const T* ps = slope + (int64_t)m * N + n;
+    for (; m + (kDepth - 1) * rows < m1; m += kDepth * rows) {
+      P g[kDepth], sl[kDepth];
 #pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = Elem<T>::load(g.e + e);
-      if (z) {
-        const P zz = *reinterpret_cast<const P*>(z + (int64_t)m * N + n);
-#pragma unroll
-        for (int e = 0; e < V; ++e) d[e] *= act_slope<sizeof(T) == 2>(Elem<T>::load(zz.e + e), act);
-        if (dz.p) store_operand<T, V>(dz, (int64_t)m * dz.ld + n, d);
+      for (int i = 0; i < kDepth; ++i) {
+        g[i] = *reinterpret_cast<const P*>(pg);
+        if (SLOPE) sl[i] = *reinterpret_cast<const P*>(ps);
+        pg += (int64_t)rows * ldy;
+        ps += (int64_t)rows * N;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += d[e];
+      for (int i = 0; i < kDepth; ++i) row(m + i * rows, g[i], sl[i]);
+    }
+    for (; m < m1; m += rows) {
+      const P g = *reinterpret_cast<const P*>(pg);
+      P sl{};
+      if (SLOPE) sl = *reinterpret_cast<const P*>(ps);
+      row(m, g, sl);
+      pg += (int64_t)rows * ldy;
+      ps += (int64_t)rows * N;
     }
   }
   if (!part) return;
 #pragma unroll
-  for (int e = 0; e < V; ++e) s[ty][tx * V + e] = acc[e];
+  for (int e = 0; e < V; ++e) s[(ty * cols + tx) * V + e] = acc[e];
   __syncthreads();
-  for (int c = threadIdx.x; c < kDzCols * V; c += kDzCols * kDzRows) {
-    const int col = blockIdx.x * kDzCols * V + c;
+  for (int c = threadIdx.x; c < cols * V; c += kDzThreads) {
+    const int col = blockIdx.x * cols * V + c;
     if (col >= N) continue;
     float sum = 0.f;
-    for (int r = 0; r < kDzRows; ++r) sum += s[r][c];
+    for (int r = 0; r < rows; ++r) sum += s[r * cols * V + c];
     part[(int64_t)blockIdx.y * N + col] = sum;
   }
 }
@@ -116,25 +140,26 @@ __global__ void __launch_bounds__(256) k_col_sum(const float* part, int chunks, 
   }
 }
 
-int dz_chunks(int M, int N, int V) {
-  // about four blocks per SM, chunks of 32 rows at least
-  const int cols = (N + kDzCols * V - 1) / (kDzCols * V);
-  int c = (148 * 4 + cols - 1) / cols;
-  const int most = (M + 31) / 32;
-  if (c > most) c = most;
-  return c > kDzChunks ? kDzChunks : c;
-}
-
 template <typename T, int V>
 void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cudaStream_t st) {
   const int M = (int)a.rows, N = a.out_features;
-  const int most = dz_chunks(M, N, V);
+  int cols = 32;
+  while (cols < kDzThreads && cols * V < N) cols *= 2;
+  const int blocks_x = (N + cols * V - 1) / (cols * V);
+  // six blocks per SM, so that the last ones leave little idle; at least 32 rows per chunk
+  int most = (148 * 6 + blocks_x - 1) / blocks_x;
+  if (most > kDzChunks) most = kDzChunks;
+  if (most > (M + 31) / 32) most = (M + 31) / 32;
   const int chunk = (M + most - 1) / most;
   const int chunks = (M + chunk - 1) / chunk;
-  const dim3 grid((N + kDzCols * V - 1) / (kDzCols * V), chunks);
-  MURM_LAUNCH("linear_dz", (k_dz<T, V>), grid, kDzCols * kDzRows, 0, st, static_cast<const T*>(a.grad_out), a.go_stride,
-              a.activation == MURM_ACT_NONE ? (const T*)nullptr : static_cast<const T*>(a.preact), M, N, a.activation,
-              chunk, dz, part);
+  const dim3 grid(blocks_x, chunks);
+  const T* dy = static_cast<const T*>(a.grad_out);
+  if (a.activation == MURM_ACT_NONE)
+    MURM_LAUNCH("linear_col_part", (k_dz<T, V, false>), grid, kDzThreads, 0, st, dy, a.go_stride,
+                (const T*)nullptr, M, N, cols, chunk, dz, part);
+  else
+    MURM_LAUNCH("linear_dz", (k_dz<T, V, true>), grid, kDzThreads, 0, st, dy, a.go_stride,
+                static_cast<const T*>(a.slope), M, N, cols, chunk, dz, part);
   if (part)
     MURM_LAUNCH("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 256, 0, st, (const float*)part, chunks, N,
                 static_cast<T*>(a.grad_bias));
@@ -143,7 +168,7 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
 template <typename T>
 void run_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.grad_out) | reinterpret_cast<uintptr_t>(a.preact);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.grad_out) | reinterpret_cast<uintptr_t>(a.slope);
   if (a.out_features % V == 0 && a.go_stride % V == 0 && bits % 16 == 0)
     launch_dz<T, V>(a, dz, part, st);
   else
@@ -187,7 +212,7 @@ murm_status check_fwd(const murm_linear_args* a) {
   if (murm_status s = check_mat("weight", a->weight, a->w_stride, a->in_features, a->dtype, false)) return s;
   if (murm_status s = check_mat("bias", a->bias, a->out_features, a->out_features, a->dtype, true)) return s;
   if (murm_status s = check_mat("residual", a->residual, a->r_stride, a->out_features, a->dtype, true)) return s;
-  if (murm_status s = check_mat("preact", a->preact, a->out_features, a->out_features, a->dtype, true)) return s;
+  if (murm_status s = check_mat("slope", a->slope, a->out_features, a->out_features, a->dtype, true)) return s;
   return check_mat("out", a->out, a->out_stride, a->out_features, a->dtype, false);
 }
 
@@ -201,7 +226,7 @@ murm_status check_bwd(const murm_linear_bwd_args* a) {
   if (a->rows == 0) return MURM_OK;
   if (murm_status s = check_mat("x", a->x, a->x_stride, in, dt, a->grad_weight == nullptr)) return s;
   if (murm_status s = check_mat("weight", a->weight, a->w_stride, in, dt, a->grad_x == nullptr)) return s;
-  if (murm_status s = check_mat("preact", a->preact, out, out, dt, a->activation == MURM_ACT_NONE)) return s;
+  if (murm_status s = check_mat("slope", a->slope, out, out, dt, a->activation == MURM_ACT_NONE)) return s;
   return check_mat("grad_out", a->grad_out, a->go_stride, out, dt, false);
 }
 
@@ -263,7 +288,7 @@ FwdPlan plan_fwd(const murm_linear_args& a) {
   g.bias = a.bias;
   g.res = a.residual; g.ldr = a.r_stride;
   g.out = a.out; g.ldo = a.out_stride;
-  g.preact = a.preact;
+  g.slope = a.slope;
   g.act = a.activation;
   p.gemm_at = p.l.take(gemm_workspace(g));
   return p;

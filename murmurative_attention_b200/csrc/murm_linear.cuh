@@ -25,7 +25,7 @@ struct Gemm {
   const void* bias;
   const void* res; int64_t ldr;
   void* out; int64_t ldo;
-  void* preact;  // [M][N] contiguous, or NULL
+  void* slope;   // [M][N] contiguous: act'(z), or NULL
   int act;       // murm_activation
 };
 size_t gemm_workspace(const Gemm& g);
@@ -96,45 +96,40 @@ __device__ __forceinline__ float relu_(float z) {
   return r;
 }
 
+// act(z) and, beside it, its slope there (the forward saves slopes for the backward: they share
+// the costly part, and a rounded slope is nearer than the slope at a rounded z). The compiler drops
+// the slope where it is not used.
 template <bool FAST>
-__device__ __forceinline__ float act_value(float z, int act) {
+__device__ __forceinline__ float act_value(float z, int act, float& slope) {
   switch (act) {
-    case MURM_ACT_RELU: return relu_(z);
-    case MURM_ACT_SILU: return z * silu_sigmoid<FAST>(z);
-    case MURM_ACT_GELU:
+    case MURM_ACT_RELU:
+      slope = z > 0.f ? 1.f : 0.f;
+      return relu_(z);
+    case MURM_ACT_SILU: {
+      const float s = silu_sigmoid<FAST>(z), y = z * s;
+      slope = fmaf(y, 1.f - s, s);
+      return y;
+    }
+    case MURM_ACT_GELU: {
       if (FAST) {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|); past 30 the second term is 0
         float e;
         const float a = fminf(fabsf(z), 30.f);
-        return fmaf(-a, normal_tail(a, e), relu_(z));
+        const float q = normal_tail(a, e);
+        slope = fmaf(z * kInvSqrt2Pi, e, z < 0.f ? q : 1.f - q);
+        return fmaf(-a, q, relu_(z));
       }
-      return 0.5f * z * (1.f + erff(z * kSqrtHalf));
-    case MURM_ACT_GELU_TANH:  // 0.5 (1 + tanh u) = sigmoid(2u)
-      return z * sigmoid_<FAST>(z, kTanhA, kTanhB);
+      const float c = 0.5f * (1.f + erff(z * kSqrtHalf));
+      slope = c + z * kInvSqrt2Pi * expf(-0.5f * z * z);
+      return z * c;
+    }
+    case MURM_ACT_GELU_TANH: {  // 0.5 (1 + tanh u) = sigmoid(2u)
+      const float s = sigmoid_<FAST>(z, kTanhA, kTanhB), y = z * s;
+      slope = fmaf(y * (1.f - s), fmaf(3.f * kTanhB, fminf(z * z, 1e6f), kTanhA), s);
+      return y;
+    }
   }
+  slope = 1.f;
   return z;
-}
-// d act / dz
-template <bool FAST>
-__device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-    case MURM_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case MURM_ACT_SILU: {
-      const float s = silu_sigmoid<FAST>(z);
-      return s * (1.f + z * (1.f - s));
-    }
-    case MURM_ACT_GELU:
-      if (FAST) {
-        float e;
-        const float q = normal_tail(fabsf(z), e);
-        return fmaf(z * kInvSqrt2Pi, e, z < 0.f ? q : 1.f - q);
-      }
-      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expf(-0.5f * z * z);
-    case MURM_ACT_GELU_TANH: {
-      const float s = sigmoid_<FAST>(z, kTanhA, kTanhB);
-      return s + z * s * (1.f - s) * (kTanhA + 3.f * kTanhB * z * z);
-    }
-  }
-  return 1.f;
 }
 
 // The three bf16 terms of an fp32 value, each the leading 8 bits of what is left (cut, so that no

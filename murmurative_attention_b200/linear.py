@@ -38,15 +38,15 @@ def _workspace(fn, args, dev) -> Optional[torch.Tensor]:
 
 
 def _forward(x, weight, bias, residual, act, save):
-    """x [M, K], weight [N, K], residual [M, N] -> (out [M, N], preact or None)."""
+    """x [M, K], weight [N, K], residual [M, N] -> (out [M, N], slope or None)."""
     lib = _lib.load_library()
     x, weight = _rows(x), _rows(weight)
     M, K = x.shape
     N = weight.shape[0]
     out = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    preact = torch.empty_like(out) if save and act else None
+    slope = torch.empty_like(out) if save and act else None
     if not out.numel():
-        return out, preact
+        return out, slope
     if bias is not None:
         bias = bias.contiguous()
     a = _lib.LinearArgs(M, K, N, dtype_code(x, "x"), act, x.data_ptr(), _stride(x), weight.data_ptr(),
@@ -55,14 +55,14 @@ def _forward(x, weight, bias, residual, act, save):
         residual = _rows(residual)
         a.residual, a.r_stride = residual.data_ptr(), _stride(residual)
     a.out, a.out_stride = out.data_ptr(), N
-    if preact is not None:
-        a.preact = preact.data_ptr()
+    if slope is not None:
+        a.slope = slope.data_ptr()
     ws = _workspace(lib.murm_linear_workspace, a, x.device)  # noqa: F841  (alive until the call is enqueued)
     call(lib.murm_linear_fwd, a, x.device)
-    return out, preact
+    return out, slope
 
 
-def _backward(x, weight, preact, go, act, need_x, need_w, need_b):
+def _backward(x, weight, slope, go, act, need_x, need_w, need_b):
     lib = _lib.load_library()
     x, weight, go = _rows(x), _rows(weight), _rows(go.to(x.dtype))
     M, K = x.shape
@@ -73,7 +73,7 @@ def _backward(x, weight, preact, go, act, need_x, need_w, need_b):
     gb = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
     ptr = lambda t: t.data_ptr() if t is not None else None
     a = _lib.LinearBwdArgs(M, K, N, dtype_code(x, "x"), act, x.data_ptr(), _stride(x), weight.data_ptr(),
-                           _stride(weight), ptr(preact), go.data_ptr(), _stride(go), ptr(gx), K, ptr(gw), K, ptr(gb))
+                           _stride(weight), ptr(slope), go.data_ptr(), _stride(go), ptr(gx), K, ptr(gw), K, ptr(gb))
     ws = _workspace(lib.murm_linear_bwd_workspace, a, dev)  # noqa: F841
     call(lib.murm_linear_bwd, a, dev)
     return gx, gw, gb
@@ -82,19 +82,19 @@ def _backward(x, weight, preact, go, act, need_x, need_w, need_b):
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        out, preact = _forward(x, weight, bias, residual, act, True)
-        ctx.save_for_backward(x, weight, preact)
+        out, slope = _forward(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, slope)
         ctx.act = act
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        x, weight, preact = ctx.saved_tensors
+        x, weight, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
         gx = gw = gb = None
         if need[0] or need[1] or need[2]:
-            gx, gw, gb = _backward(x, weight, preact, go, ctx.act, need[0], need[1], need[2])
+            gx, gw, gb = _backward(x, weight, slope, go, ctx.act, need[0], need[1], need[2])
         return gx, gw, gb, go if need[3] else None, None
 
 
@@ -109,7 +109,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         activation: "none", "relu", "silu", "gelu" (error function) or "gelu_tanh".
 
     Returns [..., N]. Differentiable with respect to x, weight, bias and residual; the backward reads
-    x, weight and the pre-activation, which the forward saves in x's dtype (not for "none").
+    x, weight and the activation's slopes, which the forward saves in x's dtype (not for "none").
     """
     act = ACTIVATIONS.get(activation)
     if act is None:

@@ -7,8 +7,9 @@ Tolerances, u_T = 2^-24, 2^-11, 2^-8 the rounding of the result's type:
   4 sqrt(sum of squares of the terms) =: 4 S, so E = (K/16 + 16) 2^-23 4 S. Terms of one sign reach
   further: there S is the sum of magnitudes.
 - an activation passes z's error on with a slope of at most 1.13 and adds 2^-20 max(|z|, 1) of its own.
-- dz = dy act'(z) with z rounded to T: act'' is at most 0.8, so |dy| (0.8 (u_T |z| + E) + 2^-20), plus
-  u_T |dz| as the operand of the 16-bit products. relu's slope may differ where |z| <= E.
+- dz = dy act'(z), the slope computed from z (act'' is at most 0.8) and saved rounded to T:
+  |dy| (0.8 E + 2^-20 + u_T |slope|), plus u_T |dz| as the operand of the 16-bit products. relu's
+  slope may differ where |z| <= E.
 - sums of dz take the sum of its errors, and a column sum depth * 2^-24 of the sum of magnitudes.
 fp16 results below 2^-14 are rounded to multiples of 2^-24.
 """
@@ -67,7 +68,7 @@ def check(x, w, b, r, go, act, out, grads):
     elif act == "relu":
         Edz = torch.where(z.abs() <= E, dy.abs(), torch.zeros_like(dz))
     else:
-        Edz = dy.abs() * (0.8 * (U[dt] * z.abs() + E) + 2.0 ** -20)
+        Edz = dy.abs() * (0.8 * E + 2.0 ** -20 + U[dt] * slope.abs() + (2.0 ** -25 if dt == torch.float16 else 0))
     Eop = Edz + (U[dt] * (dz.abs() + Edz) if act != "none" else 0)
     if dt == torch.float16:
         Eop = Eop + 2.0 ** -25
