@@ -8,11 +8,16 @@
 // r is recomputed from x, so the forward saves nothing.
 //
 // Both directions read each input element once and write each output element once: the bound is
-// HBM. A row belongs to L lanes of a warp (L a power of two), each of which holds both members of
-// V pairs (two loads of V elements), so the rotation needs no exchange and the norm log2(L)
-// shuffles. A lane's pairs are the same in every row it takes, and a group of L lanes takes
-// several heads of one token: the angles (64-bit products reduced to a turn, then sincospif)
-// are formed once for all of them.
+// HBM. A row belongs to L lanes of a warp (with the norm a power of two), each of which holds both
+// members of V pairs (two loads of V elements), so the rotation needs no exchange and the norm
+// log2(L) shuffles. A lane's pairs are the same in every row it takes, and a group of L lanes takes
+// several heads of one token: the angles (64-bit products, reduced to an eighth of a turn) are formed
+// once for all of them. The norm's kernels walk over their items with a ring of asynchronous copies
+// in shared memory ahead of them; the rotation, with a third of the arithmetic, takes an item per
+// group and several rows at once.
+// Measured: norm and rotation of q and k, 8 x 8192 tokens, 16 + 4 heads of 128, bf16: 123 us
+// (671 MB, 5.5 TB/s), backward 199 us (1.0 GB, 5.1 TB/s); rotation of 2 x 23400 x 24 rows of 128:
+// 91 us (575 MB, 6.3 TB/s).
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -27,8 +32,17 @@ constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;
 constexpr int kMaxD = 256;
 constexpr int kSms = 148;
-constexpr int kBwdBlocks = kSms * 3;  // blocks of the norm's backward, each with one partial of dw
-constexpr int kRowsInFlight = 4;      // heads whose loads a forward group issues together
+// Launch shapes, by measurement (q and k of 8 x 8192 tokens, 16 + 4 heads of 128, bf16):
+// forward: 8 pairs per lane, 2 rows side by side, rings of 6, 2 blocks per SM: 123 us; 1 row 129,
+//   4 rows 137, 1 block 164, 4 pairs per lane 167 (more shuffles and addresses per byte);
+// backward: 8 pairs, 1 row, rings of 4, 2 blocks: 199 us; 4 pairs and 2 rows 214, 1 block 212.
+// rotation (2 x 23400 tokens, 24 heads of 128): 4 pairs, 4 rows, 4 blocks: 91 us; 8 pairs 93, 2 rows 99.
+constexpr int kFwdV = 8, kFwdRows = 2, kFwdDepth = 6, kFwdPerSm = 2;
+constexpr int kBwdV = 8, kBwdRows = 1, kBwdDepth = 4, kBwdPerSm = 2;
+constexpr int kRotV = 4, kRotRows = 4, kRotPerSm = 4;
+constexpr int kFwdBlocks = kSms * kFwdPerSm;
+constexpr int kBwdBlocks = kSms * kBwdPerSm;  // each with a partial of dw
+constexpr int kAngleRows = 4;  // an item's angles cost about as much as this many rows
 
 struct Rows {
   const void* x; Strides3 xs;
@@ -38,6 +52,7 @@ struct Rows {
   int w_f32;
   int heads;    // heads of the tensor
   int chunk;    // heads per group and item
+  int chunks;   // head chunks: items per token
   int items;    // (token, head chunk) items
   int blocks;   // blocks of the launch that work on this tensor
 };
@@ -61,34 +76,130 @@ template <> struct RawOf<4> { using type = uint32_t; };
 template <> struct RawOf<2> { using type = uint16_t; };
 template <typename T, int V> using Raw = typename RawOf<V * (int)sizeof(T)>::type;
 
-// The elements of one unit of a row: a[e], b[e] are the members of its e-th pair.
+// ---------------------------------------------------------------------------
+// pairs of fp32 values: one instruction for two (the kernels are close to the issue rate)
+// ---------------------------------------------------------------------------
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ f2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ void halves(f2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 neg2(f2 a) { return a ^ 0x8000000080000000ull; }
+__device__ __forceinline__ float sum2(f2 v) {
+  float lo, hi;
+  halves(v, lo, hi);
+  return lo + hi;
+}
+
+// Two neighbouring elements of a row <-> two fp32 values.
+__device__ __forceinline__ void expand(uint32_t u, float& lo, float& hi, const __nv_bfloat16*) {
+  lo = __uint_as_float(u << 16);
+  hi = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ void expand(uint32_t u, float& lo, float& hi, const __half*) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  lo = f.x;
+  hi = f.y;
+}
+__device__ __forceinline__ uint32_t shrink(float lo, float hi, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t shrink(float lo, float hi, const __half*) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The pairs of one unit of a row, two to an f2 (V = 1: one, and a zero).
+template <int V> struct Pairs { static constexpr int v = V == 1 ? 1 : V / 2; };
+
+// a, b: the first and second members of the unit's pairs. lo and hi hold its 2V elements; pairs are
+// (lo[e], hi[e]), or with INTER neighbours in the order lo, hi.
 template <typename T, int V, bool INTER>
-__device__ __forceinline__ void unpack(const Raw<T, V>& lo, const Raw<T, V>& hi, float (&a)[V], float (&b)[V]) {
-  const T* pl = reinterpret_cast<const T*>(&lo);
-  const T* ph = reinterpret_cast<const T*>(&hi);
+__device__ __forceinline__ void unpack(const Raw<T, V>& lo, const Raw<T, V>& hi, f2 (&a)[Pairs<V>::v],
+                                       f2 (&b)[Pairs<V>::v]) {
+  float x[V], y[V];  // the elements of lo, of hi
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    const uint32_t* pl = reinterpret_cast<const uint32_t*>(&lo);
+    const uint32_t* ph = reinterpret_cast<const uint32_t*>(&hi);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (INTER) {
-      a[e] = Elem<T>::load(2 * e < V ? pl + 2 * e : ph + 2 * e - V);
-      b[e] = Elem<T>::load(2 * e + 1 < V ? pl + 2 * e + 1 : ph + 2 * e + 1 - V);
-    } else {
-      a[e] = Elem<T>::load(pl + e);
-      b[e] = Elem<T>::load(ph + e);
+    for (int e = 0; e < V; e += 2) {
+      expand(pl[e / 2], x[e], x[e + 1], (const T*)nullptr);
+      expand(ph[e / 2], y[e], y[e + 1], (const T*)nullptr);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      x[e] = Elem<T>::load(reinterpret_cast<const T*>(&lo) + e);
+      y[e] = Elem<T>::load(reinterpret_cast<const T*>(&hi) + e);
+    }
+  }
+  if constexpr (V == 1) {
+    a[0] = pair(x[0], 0.f);
+    b[0] = pair(y[0], 0.f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      if (INTER) {
+        const float* q = 2 * e < V ? x + 2 * e : y + 2 * e - V;
+        a[e / 2] = pair(q[0], q[2]);
+        b[e / 2] = pair(q[1], q[3]);
+      } else {
+        a[e / 2] = pair(x[e], x[e + 1]);
+        b[e / 2] = pair(y[e], y[e + 1]);
+      }
     }
   }
 }
 template <typename T, int V, bool INTER>
-__device__ __forceinline__ void pack(const float (&a)[V], const float (&b)[V], Raw<T, V>& lo, Raw<T, V>& hi) {
-  T* pl = reinterpret_cast<T*>(&lo);
-  T* ph = reinterpret_cast<T*>(&hi);
+__device__ __forceinline__ void pack(const f2 (&a)[Pairs<V>::v], const f2 (&b)[Pairs<V>::v], Raw<T, V>& lo,
+                                     Raw<T, V>& hi) {
+  float x[V], y[V];
+  if constexpr (V == 1) {
+    float z;
+    halves(a[0], x[0], z);
+    halves(b[0], y[0], z);
+  } else {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (INTER) {
-      Elem<T>::store(2 * e < V ? pl + 2 * e : ph + 2 * e - V, a[e]);
-      Elem<T>::store(2 * e + 1 < V ? pl + 2 * e + 1 : ph + 2 * e + 1 - V, b[e]);
-    } else {
-      Elem<T>::store(pl + e, a[e]);
-      Elem<T>::store(ph + e, b[e]);
+    for (int e = 0; e < V; e += 2) {
+      if (INTER) {
+        float* q = 2 * e < V ? x + 2 * e : y + 2 * e - V;
+        halves(a[e / 2], q[0], q[2]);
+        halves(b[e / 2], q[1], q[3]);
+      } else {
+        halves(a[e / 2], x[e], x[e + 1]);
+        halves(b[e / 2], y[e], y[e + 1]);
+      }
+    }
+  }
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    uint32_t* pl = reinterpret_cast<uint32_t*>(&lo);
+    uint32_t* ph = reinterpret_cast<uint32_t*>(&hi);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      pl[e / 2] = shrink(x[e], x[e + 1], (const T*)nullptr);
+      ph[e / 2] = shrink(y[e], y[e + 1], (const T*)nullptr);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      Elem<T>::store(reinterpret_cast<T*>(&lo) + e, x[e]);
+      Elem<T>::store(reinterpret_cast<T*>(&hi) + e, y[e]);
     }
   }
 }
@@ -98,12 +209,13 @@ template <int V> struct UnitsPerLane { static constexpr int v = V >= 4 ? 1 : 4; 
 
 struct UnitAt {
   int lo, hi;  // element offsets of the unit's two runs of V elements
-  bool on;
+  bool on;     // lanes past the row's units read its last one and write nothing
 };
 template <int V, bool INTER>
-__device__ __forceinline__ UnitAt unit_at(const Params& p, int u) {
+__device__ __forceinline__ UnitAt unit_at(const Params& p, int lane_unit) {
   UnitAt r;
-  r.on = u < p.units;
+  r.on = lane_unit < p.units;
+  const int u = min(lane_unit, p.units - 1);
   if (!INTER && u < p.rot_units) {
     r.lo = u * V;
     r.hi = p.rd / 2 + u * V;
@@ -130,13 +242,23 @@ __device__ __forceinline__ double turns_of(const Params& p, int pair) {
 // cos and sin of the angle, from its turns. The product and its reduction are in 64 bits (a 32-bit
 // angle of position 100000 is off by 0.004 rad), to the nearest quarter turn: the remainder's own
 // rounding to 32 bits then moves the angle by at most 2^-28 turns (2.3e-8 rad), less than the
-// rounding of the sine itself; reduced to a half turn only it would be 2^-26 turns.
+// rounding of the sine itself; reduced to a half turn only it would be 2^-26 turns. Within the eighth
+// of a turn that is left (x = pi/4 at most) the Taylor series to x^9 and x^10 leave x^11 / 11! < 2e-9
+// and x^12 / 12! < 2e-10.
 __device__ __forceinline__ void cos_sin(double pos, double turns, float& c, float& s) {
   double t = pos * turns;
   t -= rint(t);
   const double quarter = rint(4.0 * t);
-  float c0, s0;
-  sincospif(2.0f * (float)(t - 0.25 * quarter), &s0, &c0);
+  const float x = 6.2831853071795865f * (float)(t - 0.25 * quarter), x2 = x * x;
+  float s0 = fmaf(x2, 1.f / 362880.f, -1.f / 5040.f);
+  s0 = fmaf(s0, x2, 1.f / 120.f);
+  s0 = fmaf(s0, x2, -1.f / 6.f);
+  s0 = fmaf(s0 * x2, x, x);
+  float c0 = fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f);
+  c0 = fmaf(c0, x2, -1.f / 720.f);
+  c0 = fmaf(c0, x2, 1.f / 24.f);
+  c0 = fmaf(c0, x2, -0.5f);
+  c0 = fmaf(c0, x2, 1.f);
   const int m = (int)quarter;  // -2..2
   const bool swap = m & 1;
   c = swap ? s0 : c0;
@@ -156,128 +278,273 @@ __device__ __forceinline__ float load_weight(const Rows& r, int i, const float*)
   return static_cast<const float*>(r.w)[i];
 }
 
-__device__ __forceinline__ float row_sum(float v, int L) {
-  for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Sums over a row's lanes, F rows side by side.
+template <int F>
+__device__ __forceinline__ void row_sums(float (&v)[F], int L) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < L) {
+#pragma unroll
+      for (int f = 0; f < F; ++f) v[f] += __shfl_xor_sync(0xffffffffu, v[f], o);
+    }
 }
 
-// What a lane keeps for the rows of one token: its units, gains and angles.
-template <typename T, int V, bool INTER, bool NORM>
+// What a lane keeps beside the rows: its units, their gains, and the angles of the current token.
+template <typename T, int V, bool INTER>
 struct LaneState {
-  static constexpr int U = UnitsPerLane<V>::v;
+  static constexpr int U = UnitsPerLane<V>::v, P = Pairs<V>::v;
   UnitAt at[U];
-  float wa[NORM ? U : 1][V], wb[NORM ? U : 1][V];
-  float c[U][V], s[U][V];
+  f2 wa[U][P], wb[U][P];
 
-  __device__ __forceinline__ void init(const Params& p, const Rows& r, int lane) {
+  __device__ __forceinline__ void gains(const Rows& r) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      at[j] = unit_at<V, INTER>(p, lane + p.L * j);
-      if (NORM) {
+      float a[2 * P], b[2 * P];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int ia = INTER ? at[j].lo + 2 * e : at[j].lo + e;
-          const int ib = INTER ? ia + 1 : at[j].hi + e;
-          wa[j][e] = r.w && at[j].on ? load_weight(r, ia, (const T*)nullptr) : 1.f;
-          wb[j][e] = r.w && at[j].on ? load_weight(r, ib, (const T*)nullptr) : 1.f;
-        }
+      for (int e = 0; e < 2 * P; ++e) {
+        const int k = e < V ? e : 0;  // V = 1 fills the idle half with a copy
+        const int ia = INTER ? at[j].lo + 2 * k : at[j].lo + k;
+        const int ib = INTER ? ia + 1 : at[j].hi + k;
+        a[e] = r.w ? load_weight(r, ia, (const T*)nullptr) : 1.f;
+        b[e] = r.w ? load_weight(r, ib, (const T*)nullptr) : 1.f;
+      }
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        wa[j][q] = pair(a[2 * q], a[2 * q + 1]);
+        wb[j][q] = pair(b[2 * q], b[2 * q + 1]);
       }
     }
   }
-  __device__ __forceinline__ void angles(const Params& p, int lane, int b, int n) {
+  // cos and sin of the pairs of unit j of token (b, n); 1 and 0 past the rotated part
+  __device__ __forceinline__ void angles(const Params& p, int lane, int b, int n, int j, f2 (&c)[P], f2 (&s)[P]) const {
+    const int u = lane + p.L * j;
+    float cs[2 * P], sn[2 * P];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int u = lane + p.L * j;
+    for (int e = 0; e < 2 * P; ++e) { cs[e] = 1.f; sn[e] = 0.f; }
+    if (u < p.rot_units) {
+      int axis = -1;
+      double pos = 0.0;
 #pragma unroll
-      for (int e = 0; e < V; ++e) { c[j][e] = 1.f; s[j][e] = 0.f; }
-      if (u < p.rot_units) {
-        int axis = -1;
-        double pos = 0.0;
+      for (int e = 0; e < V; ++e) {
+        const int pr = u * V + e;
+        const int ax = axis_of(p, pr);
+        if (ax != axis) pos = load_pos(p, b, n, ax);
+        axis = ax;
+        cos_sin(pos, turns_of(p, pr), cs[e], sn[e]);
+        if (p.inverse) sn[e] = -sn[e];
+      }
+    }
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int pair = u * V + e;
-          const int ax = axis_of(p, pair);
-          if (ax != axis) pos = load_pos(p, b, n, ax);
-          axis = ax;
-          cos_sin(pos, turns_of(p, pair), c[j][e], s[j][e]);
-          if (p.inverse) s[j][e] = -s[j][e];
+    for (int q = 0; q < P; ++q) {
+      c[q] = pair(cs[2 * q], cs[2 * q + 1]);
+      s[q] = pair(sn[2 * q], sn[2 * q + 1]);
+    }
+  }
+};
+
+// A group's walk over its rows: items (a token and `chunk` of its heads) `stride` apart, head by
+// head. Consecutive items are consecutive tokens of one head chunk: item = (c * B + b) * N + n; the
+// walk adds the stride digit by digit. Groups past the last item stay at their last one, heads past
+// the chunk's last at that, so that no load has a condition of its own; neither writes.
+struct Walk {
+  int c, b, n;     // head chunk, batch, token
+  int dc, db, dn;  // the stride's digits
+  int h, count;    // head within the chunk, heads in it
+  bool live;
+  __device__ __forceinline__ void start(const Params& p, const Rows& r, int item, int stride) {
+    live = item < r.items;
+    if (!live) item = r.items - 1;
+    c = item / p.N;
+    n = item - c * p.N;
+    b = c % p.B;
+    c /= p.B;
+    dc = stride / p.N;
+    dn = stride - dc * p.N;
+    db = dc % p.B;
+    dc /= p.B;
+    enter(r);
+  }
+  __device__ __forceinline__ void enter(const Rows& r) {
+    h = 0;
+    count = min(r.chunk, r.heads - c * r.chunk);
+  }
+  // F rows on (F divides the chunk); true when that begins another item.
+  template <int F>
+  __device__ __forceinline__ bool step(const Params& p, const Rows& r) {
+    h += F;
+    if (h < r.chunk) return false;
+    int c1 = c + dc, b1 = b + db, n1 = n + dn;
+    if (n1 >= p.N) { n1 -= p.N; ++b1; }
+    if (b1 >= p.B) { b1 -= p.B; ++c1; }
+    live = live && c1 < r.chunks;
+    if (live) { c = c1; b = b1; n = n1; }
+    enter(r);
+    return true;
+  }
+  __device__ __forceinline__ const void* position(const Params& p) const {
+    const int64_t at = b * p.ps[0] + n * p.ps[1];
+    return static_cast<const char*>(p.pos) + at * (p.pos_type == MURM_POS_I64 ? 8 : 4);
+  }
+};
+
+__device__ __forceinline__ void async_copy(uint32_t dst, const void* src, uint4*) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_copy(uint32_t dst, const void* src, uint2*) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() {  // all but the newest N groups have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The rows of A arrays (x; x and dy) on their way to a lane: a ring of S slots in shared memory that
+// only this lane writes and reads, filled by asynchronous copies S - F rows ahead, so that the bytes
+// in flight cost no registers and need no barrier. F rows are taken at a time. Without wide accesses
+// (V = 1) rows are loaded when they are due.
+template <typename T, int V, int U, int A, int S, int F>
+struct Ring {
+  using R = Raw<T, V>;
+  static constexpr bool kAsync = V >= 4;
+  static constexpr uint32_t kHalf = kThreads * sizeof(R);  // the block's lanes side by side
+  static constexpr uint32_t kSlot = A * 2 * kHalf;
+  static constexpr int kBytes = kAsync ? S * (int)kSlot : 0;
+  const Params& p;
+  const Rows& r;
+  const UnitAt (&at)[U];
+  const T* row[A];
+  Walk w;            // the next row to fetch
+  int left;
+  uint32_t smem, slot;  // this lane's place in slot 0; the slot to fill next, in bytes
+
+  __device__ __forceinline__ Ring(const Params& p_, const Rows& r_, const UnitAt (&at_)[U], void* sm, int first,
+                                  int stride, int total)
+      : p(p_), r(r_), at(at_), left(total), smem(sm100::smem_u32(sm) + threadIdx.x * (uint32_t)sizeof(R)), slot(0) {
+    w.start(p, r, first, stride);
+    enter();
+    if constexpr (kAsync)
+      for (int i = 0; i < S - F; ++i) fetch();
+  }
+  __device__ __forceinline__ void enter() {
+    row[0] = row_ptr(static_cast<const T*>(r.x), r.xs, w.b, w.c * r.chunk, w.n);
+    if (A == 2) row[A - 1] = row_ptr(static_cast<const T*>(r.g), r.gs, w.b, w.c * r.chunk, w.n);
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(w.position(p)));
+  }
+  __device__ __forceinline__ void step() {
+    if (w.template step<1>(p, r)) {
+      enter();
+    } else if (w.h < w.count) {
+      row[0] += r.xs.s[1];
+      if (A == 2) row[A - 1] += r.gs.s[1];
+    }
+  }
+  __device__ __forceinline__ void fetch() {
+    if (left > 0) {
+      --left;
+#pragma unroll
+      for (int a = 0; a < A; ++a) {
+        async_copy(smem + slot + a * 2 * kHalf, row[a] + at[0].lo, (R*)nullptr);
+        async_copy(smem + slot + (a * 2 + 1) * kHalf, row[a] + at[0].hi, (R*)nullptr);
+      }
+      step();
+    }
+    async_commit();
+    slot += kSlot;
+    if (slot == S * kSlot) slot = 0;
+  }
+  // The next F rows' units.
+  __device__ __forceinline__ void next(void* sm, R (&lo)[F][A][U], R (&hi)[F][A][U]) {
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int f = 0; f < F; ++f) fetch();
+      async_wait<S - F>();
+      const uint8_t* s = static_cast<const uint8_t*>(sm) + threadIdx.x * sizeof(R);
+      uint32_t at_slot = slot;  // all slots are taken: the next one to fill holds the oldest row
+#pragma unroll
+      for (int f = 0; f < F; ++f, at_slot += kSlot) {
+        if (at_slot == S * kSlot) at_slot = 0;
+#pragma unroll
+        for (int a = 0; a < A; ++a) {
+          lo[f][a][0] = *reinterpret_cast<const R*>(s + at_slot + a * 2 * kHalf);
+          hi[f][a][0] = *reinterpret_cast<const R*>(s + at_slot + (a * 2 + 1) * kHalf);
         }
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+#pragma unroll
+        for (int a = 0; a < A; ++a)
+#pragma unroll
+          for (int j = 0; j < U; ++j) {
+            lo[f][a][j] = __ldg(reinterpret_cast<const R*>(row[a] + at[j].lo));
+            hi[f][a][j] = __ldg(reinterpret_cast<const R*>(row[a] + at[j].hi));
+          }
+        step();
       }
     }
   }
 };
 
-template <typename T, int V, bool INTER, bool NORM>
-__global__ void __launch_bounds__(kThreads) k_rope_fwd(const __grid_constant__ Params p) {
-  constexpr int U = UnitsPerLane<V>::v;
-  constexpr int F = U == 1 ? kRowsInFlight : 1;
+// The rounds of a block over its tensor's items.
+__device__ __forceinline__ int block_rounds(const Rows& r, int first, int stride) {
+  return first < r.items ? (r.items - first + stride - 1) / stride : 0;
+}
+
+// The rotation alone: an item per group, its first heads' loads on their way while the angles are
+// formed. No sums over the row, so L is the row's number of units whatever it is (9 lanes for a row of
+// 72: 26 us for 516096 rows of bf16; in groups of 16 lanes 37 us).
+template <typename T, int V, bool INTER>
+__global__ void __launch_bounds__(kThreads, kRotPerSm) k_rotate(const __grid_constant__ Params p) {
+  constexpr int U = UnitsPerLane<V>::v, F = U == 1 ? kRotRows : 1, P = Pairs<V>::v;
   using R = Raw<T, V>;
-  const bool second = blockIdx.x >= p.t[0].blocks;
-  const Rows& r = p.t[second];
-  const int block = blockIdx.x - (second ? p.t[0].blocks : 0);
-  const int lane = threadIdx.x & (p.L - 1);
-  const int item = block * (kThreads / p.L) + threadIdx.x / p.L;
-  // consecutive groups take consecutive tokens of one head chunk
-  const int tokens = p.B * p.N;
-  const bool live = item < r.items;
-  const int chunk = live ? item / tokens : 0;
-  const int bn = live ? item - chunk * tokens : 0;
-  const int b = bn / p.N, n = bn - b * p.N;
-  LaneState<T, V, INTER, NORM> st;
-  st.init(p, r, lane);
-  st.angles(p, lane, b, n);
-  const float inv_d = 1.f / (float)p.d;
-  const T* x = row_ptr(static_cast<const T*>(r.x), r.xs, b, 0, n);
-  T* y = row_ptr(static_cast<T*>(r.y), r.ys, b, 0, n);
-  const int h0 = chunk * r.chunk;
-  const int h1 = min(r.heads, h0 + r.chunk);
-  for (int hb = 0; hb < r.chunk; hb += F) {  // the same trip count in every lane: the norm shuffles
-    R lo[F][U], hi[F][U];
+  const Rows& r = p.t[0];
+  const int groups = kThreads / p.L, group = threadIdx.x / p.L, lane = threadIdx.x - group * p.L;
+  if (group >= groups) return;
+  LaneState<T, V, INTER> st;
+#pragma unroll
+  for (int j = 0; j < U; ++j) st.at[j] = unit_at<V, INTER>(p, lane + p.L * j);
+  Walk w;
+  w.start(p, r, blockIdx.x * groups + group, 0);
+  const T* x = row_ptr(static_cast<const T*>(r.x), r.xs, w.b, w.c * r.chunk, w.n);
+  T* y = row_ptr(static_cast<T*>(r.y), r.ys, w.b, w.c * r.chunk, w.n);
+  R lo[F][U], hi[F][U];
+  auto load = [&](int h) {  // past the last head: that one again
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-      const int h = h0 + hb + f;
-      const T* row = x + (int64_t)h * r.xs.s[1];
+      const T* row = x + (int64_t)min(h + f, w.count - 1) * r.xs.s[1];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        lo[f][j] = R{};
-        hi[f][j] = R{};
-        if (live && h < h1 && st.at[j].on) {
-          lo[f][j] = __ldg(reinterpret_cast<const R*>(row + st.at[j].lo));
-          hi[f][j] = __ldg(reinterpret_cast<const R*>(row + st.at[j].hi));
-        }
+        lo[f][j] = __ldg(reinterpret_cast<const R*>(row + st.at[j].lo));
+        hi[f][j] = __ldg(reinterpret_cast<const R*>(row + st.at[j].hi));
       }
     }
+  };
+  load(0);
+  f2 c[U][P], s[U][P], ns[U][P];
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    st.angles(p, lane, w.b, w.n, j, c[j], s[j]);
+#pragma unroll
+    for (int q = 0; q < P; ++q) ns[j][q] = neg2(s[j][q]);
+  }
+  for (int h = 0; h < w.count; h += F) {
+    if (h > 0) load(h);
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-      const int h = h0 + hb + f;
-      float a[U][V], bb[U][V];
-      float ss = 0.f;
+      T* row = y + (int64_t)(h + f) * r.ys.s[1];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        unpack<T, V, INTER>(lo[f][j], hi[f][j], a[j], bb[j]);
-        if (NORM) {
+        f2 xa[P], xb[P], ya[P], yb[P];
+        unpack<T, V, INTER>(lo[f][j], hi[f][j], xa, xb);
 #pragma unroll
-          for (int e = 0; e < V; ++e) ss += a[j][e] * a[j][e] + bb[j][e] * bb[j][e];
+        for (int q = 0; q < P; ++q) {
+          ya[q] = fma2(xa[q], c[j][q], mul2(xb[q], ns[j][q]));
+          yb[q] = fma2(xa[q], s[j][q], mul2(xb[q], c[j][q]));
         }
-      }
-      float rn = 1.f;
-      if (NORM) rn = rsqrtf(row_sum(ss, p.L) * inv_d + p.eps);
-      T* row = y + (int64_t)h * r.ys.s[1];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float ua = a[j][e], ub = bb[j][e];
-          if (NORM) {
-            ua *= rn * st.wa[j][e];
-            ub *= rn * st.wb[j][e];
-          }
-          a[j][e] = ua * st.c[j][e] - ub * st.s[j][e];
-          bb[j][e] = ua * st.s[j][e] + ub * st.c[j][e];
-        }
-        if (live && h < h1 && st.at[j].on) {
+        if (w.live && h + f < w.count && st.at[j].on) {
           R l, u;
-          pack<T, V, INTER>(a[j], bb[j], l, u);
+          pack<T, V, INTER>(ya, yb, l, u);
           *reinterpret_cast<R*>(row + st.at[j].lo) = l;
           *reinterpret_cast<R*>(row + st.at[j].hi) = u;
         }
@@ -286,104 +553,184 @@ __global__ void __launch_bounds__(kThreads) k_rope_fwd(const __grid_constant__ P
   }
 }
 
-// The norm's backward. A group strides over items of one tensor and sums dw of its own pairs in
-// registers; the block adds its groups up in shared memory, in group order, into one partial.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kThreads) k_norm_rope_bwd(const __grid_constant__ Params p) {
-  constexpr int U = UnitsPerLane<V>::v;
-  constexpr int F = U == 1 ? 2 : 1;
+__global__ void __launch_bounds__(kThreads, kFwdPerSm) k_norm_rope_fwd(const __grid_constant__ Params p) {
+  constexpr int U = UnitsPerLane<V>::v, F = U == 1 ? kFwdRows : 1;
   using R = Raw<T, V>;
-  extern __shared__ float s_dw[];  // [groups][d]
+  extern __shared__ __align__(16) uint8_t smem[];
   const bool second = blockIdx.x >= p.t[0].blocks;
   const Rows& r = p.t[second];
   const int block = blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & (p.L - 1);
-  const int groups = kThreads / p.L, group = threadIdx.x / p.L;
-  const int tokens = p.B * p.N;
-  LaneState<T, V, INTER, true> st;
-  st.init(p, r, lane);
+  const int groups = kThreads / p.L, group = threadIdx.x / p.L, stride = r.blocks * groups;
+  const int total = block_rounds(r, block * groups, stride) * r.chunk;  // rows per group, uniform in the block
+  constexpr int P = Pairs<V>::v;
+  LaneState<T, V, INTER> st;
+#pragma unroll
+  for (int j = 0; j < U; ++j) st.at[j] = unit_at<V, INTER>(p, lane + p.L * j);
+  Ring<T, V, U, 1, kFwdDepth, F> ring(p, r, st.at, smem, block * groups + group, stride, total);
+  st.gains(r);
   const float inv_d = 1.f / (float)p.d;
-  float da[U][V], db[U][V];
+  // y = (x r w) turned: a' = r (xa (wa cos) - xb (wb sin)), b' = r (xa (wa sin) + xb (wb cos)); the
+  // four products of gain and angle hold for all of a token's heads
+  f2 aa[U][P], ab[U][P], ba[U][P], bb[U][P];
+  Walk w;
+  w.start(p, r, block * groups + group, stride);
+  T* row = nullptr;
+  for (int i = 0; i < total; i += F) {
+    if (w.h == 0) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        f2 c[P], s[P];
+        st.angles(p, lane, w.b, w.n, j, c, s);
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          aa[j][q] = mul2(st.wa[j][q], c[q]);
+          ab[j][q] = neg2(mul2(st.wb[j][q], s[q]));
+          ba[j][q] = mul2(st.wa[j][q], s[q]);
+          bb[j][q] = mul2(st.wb[j][q], c[q]);
+        }
+      }
+      row = row_ptr(static_cast<T*>(r.y), r.ys, w.b, w.c * r.chunk, w.n);
+    }
+    R lo[F][1][U], hi[F][1][U];
+    ring.next(smem, lo, hi);
+    f2 xa[F][U][P], xb[F][U][P];
+    float ss[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      ss[f] = 0.f;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        unpack<T, V, INTER>(lo[f][0][j], hi[f][0][j], xa[f][j], xb[f][j]);
+        f2 q2 = 0;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          q2 = fma2(xa[f][j][q], xa[f][j][q], q2);
+          q2 = fma2(xb[f][j][q], xb[f][j][q], q2);
+        }
+        ss[f] += st.at[j].on ? sum2(q2) : 0.f;
+      }
+    }
+    row_sums<F>(ss, p.L);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const f2 rn = both(rsqrtf(ss[f] * inv_d + p.eps));
+      const bool on = w.live && w.h + f < w.count;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        f2 ya[P], yb[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const f2 u = mul2(xa[f][j][q], rn), v = mul2(xb[f][j][q], rn);
+          ya[q] = fma2(u, aa[j][q], mul2(v, ab[j][q]));
+          yb[q] = fma2(u, ba[j][q], mul2(v, bb[j][q]));
+        }
+        if (on && st.at[j].on) {
+          R l, u;
+          pack<T, V, INTER>(ya, yb, l, u);
+          *reinterpret_cast<R*>(row + st.at[j].lo) = l;
+          *reinterpret_cast<R*>(row + st.at[j].hi) = u;
+        }
+      }
+      row += r.ys.s[1];
+    }
+    w.template step<F>(p, r);
+  }
+}
+
+// The norm's backward. A group sums dw of its own pairs in registers over all its rows; the block
+// adds its groups up in shared memory, in group order, into one partial.
+template <typename T, int V, bool INTER>
+__global__ void __launch_bounds__(kThreads, kBwdPerSm) k_norm_rope_bwd(const __grid_constant__ Params p) {
+  constexpr int U = UnitsPerLane<V>::v, F = U == 1 ? kBwdRows : 1;
+  using R = Raw<T, V>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const bool second = blockIdx.x >= p.t[0].blocks;
+  const Rows& r = p.t[second];
+  const int block = blockIdx.x - (second ? p.t[0].blocks : 0);
+  const int lane = threadIdx.x & (p.L - 1);
+  const int groups = kThreads / p.L, group = threadIdx.x / p.L, stride = r.blocks * groups;
+  const int total = block_rounds(r, block * groups, stride) * r.chunk;
+  constexpr int P = Pairs<V>::v;
+  LaneState<T, V, INTER> st;
+#pragma unroll
+  for (int j = 0; j < U; ++j) st.at[j] = unit_at<V, INTER>(p, lane + p.L * j);
+  Ring<T, V, U, 2, kBwdDepth, F> ring(p, r, st.at, smem, block * groups + group, stride, total);
+  st.gains(r);
+  const float inv_d = 1.f / (float)p.d;
+  f2 da[U][P], db[U][P], c[U][P], s[U][P];
 #pragma unroll
   for (int j = 0; j < U; ++j)
 #pragma unroll
-    for (int e = 0; e < V; ++e) da[j][e] = db[j][e] = 0.f;
-  for (int base = block * groups; base < r.items; base += r.blocks * groups) {  // uniform in the block
-    const int item = base + group;
-    const bool live = item < r.items;
-    const int chunk = live ? item / tokens : 0;
-    const int bn = live ? item - chunk * tokens : 0;
-    const int b = bn / p.N, n = bn - b * p.N;
-    st.angles(p, lane, b, n);
-    const T* x = row_ptr(static_cast<const T*>(r.x), r.xs, b, 0, n);
-    const T* g = row_ptr(static_cast<const T*>(r.g), r.gs, b, 0, n);
-    T* y = row_ptr(static_cast<T*>(r.y), r.ys, b, 0, n);
-    const int h0 = chunk * r.chunk;
-    const int h1 = min(r.heads, h0 + r.chunk);
-    for (int hb = 0; hb < r.chunk; hb += F) {
-      R xl[F][U], xh[F][U], gl[F][U], gh[F][U];
+    for (int q = 0; q < P; ++q) da[j][q] = db[j][q] = 0;
+  Walk w;
+  w.start(p, r, block * groups + group, stride);
+  T* row = nullptr;
+  for (int i = 0; i < total; i += F) {
+    if (w.h == 0) {
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        const int h = h0 + hb + f;
-        const T* xr = x + (int64_t)h * r.xs.s[1];
-        const T* gr = g + (int64_t)h * r.gs.s[1];
+      for (int j = 0; j < U; ++j) st.angles(p, lane, w.b, w.n, j, c[j], s[j]);
+      row = row_ptr(static_cast<T*>(r.y), r.ys, w.b, w.c * r.chunk, w.n);
+    }
+    R lo[F][2][U], hi[F][2][U];
+    ring.next(smem, lo, hi);
+    f2 xa[F][U][P], xb[F][U][P], ga[F][U][P], gb[F][U][P];
+    float ss[F], sx[F];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-          xl[f][j] = R{}; xh[f][j] = R{}; gl[f][j] = R{}; gh[f][j] = R{};
-          if (live && h < h1 && st.at[j].on) {
-            xl[f][j] = __ldg(reinterpret_cast<const R*>(xr + st.at[j].lo));
-            xh[f][j] = __ldg(reinterpret_cast<const R*>(xr + st.at[j].hi));
-            gl[f][j] = __ldg(reinterpret_cast<const R*>(gr + st.at[j].lo));
-            gh[f][j] = __ldg(reinterpret_cast<const R*>(gr + st.at[j].hi));
-          }
+    for (int f = 0; f < F; ++f) {
+      ss[f] = sx[f] = 0.f;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        unpack<T, V, INTER>(lo[f][0][j], hi[f][0][j], xa[f][j], xb[f][j]);
+        unpack<T, V, INTER>(lo[f][1][j], hi[f][1][j], ga[f][j], gb[f][j]);
+        f2 q2 = 0, x2 = 0;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {  // g = R^T dy
+          const f2 u = ga[f][j][q], v = gb[f][j][q];
+          ga[f][j][q] = fma2(u, c[j][q], mul2(v, s[j][q]));
+          gb[f][j][q] = fma2(v, c[j][q], mul2(neg2(u), s[j][q]));
+          q2 = fma2(xa[f][j][q], xa[f][j][q], q2);
+          q2 = fma2(xb[f][j][q], xb[f][j][q], q2);
+          x2 = fma2(mul2(ga[f][j][q], st.wa[j][q]), xa[f][j][q], x2);
+          x2 = fma2(mul2(gb[f][j][q], st.wb[j][q]), xb[f][j][q], x2);
         }
+        ss[f] += st.at[j].on ? sum2(q2) : 0.f;
+        sx[f] += st.at[j].on ? sum2(x2) : 0.f;
       }
+    }
+    row_sums<F>(ss, p.L);
+    row_sums<F>(sx, p.L);
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        const int h = h0 + hb + f;
-        float xa[U][V], xb[U][V], ga[U][V], gb[U][V];
-        float ss = 0.f, sx = 0.f;
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          unpack<T, V, INTER>(xl[f][j], xh[f][j], xa[j], xb[j]);
-          unpack<T, V, INTER>(gl[f][j], gh[f][j], ga[j], gb[j]);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {  // g = R^T dy
-            const float u = ga[j][e], v = gb[j][e];
-            ga[j][e] = u * st.c[j][e] + v * st.s[j][e];
-            gb[j][e] = v * st.c[j][e] - u * st.s[j][e];
-            ss += xa[j][e] * xa[j][e] + xb[j][e] * xb[j][e];
-            sx += ga[j][e] * st.wa[j][e] * xa[j][e] + gb[j][e] * st.wb[j][e] * xb[j][e];
-          }
-        }
-        ss = row_sum(ss, p.L);
-        sx = row_sum(sx, p.L);
-        const float rn = rsqrtf(ss * inv_d + p.eps);
-        const float k = rn * rn * (sx * inv_d);
-        const bool on = live && h < h1;
-        T* row = y + (int64_t)h * r.ys.s[1];
+    for (int f = 0; f < F; ++f) {
+      const float rn = rsqrtf(ss[f] * inv_d + p.eps);
+      const f2 r2 = both(rn), k2 = both(-rn * rn * (sx[f] * inv_d));
+      if (w.live && w.h + f < w.count) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
+          f2 ya[P], yb[P];
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            if (on) {  // rows past the end would add 0 * rsqrt(eps), NaN when eps is 0
-              da[j][e] += ga[j][e] * (xa[j][e] * rn);
-              db[j][e] += gb[j][e] * (xb[j][e] * rn);
-            }
-            ga[j][e] = rn * (ga[j][e] * st.wa[j][e] - xa[j][e] * k);
-            gb[j][e] = rn * (gb[j][e] * st.wb[j][e] - xb[j][e] * k);
+          for (int q = 0; q < P; ++q) {
+            da[j][q] = fma2(ga[f][j][q], mul2(xa[f][j][q], r2), da[j][q]);
+            db[j][q] = fma2(gb[f][j][q], mul2(xb[f][j][q], r2), db[j][q]);
+            ya[q] = mul2(r2, fma2(xa[f][j][q], k2, mul2(ga[f][j][q], st.wa[j][q])));
+            yb[q] = mul2(r2, fma2(xb[f][j][q], k2, mul2(gb[f][j][q], st.wb[j][q])));
           }
-          if (on && st.at[j].on) {
+          if (st.at[j].on) {
             R l, u;
-            pack<T, V, INTER>(ga[j], gb[j], l, u);
+            pack<T, V, INTER>(ya, yb, l, u);
             *reinterpret_cast<R*>(row + st.at[j].lo) = l;
             *reinterpret_cast<R*>(row + st.at[j].hi) = u;
           }
         }
       }
+      row += r.ys.s[1];
     }
+    w.template step<F>(p, r);
   }
   if (!p.part) return;
+  float* s_dw = reinterpret_cast<float*>(smem);  // [groups][d], over the rings
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < U; ++j) {
     if (!st.at[j].on) continue;
@@ -391,8 +738,11 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope_bwd(const __grid_constan
     for (int e = 0; e < V; ++e) {
       const int ia = INTER ? st.at[j].lo + 2 * e : st.at[j].lo + e;
       const int ib = INTER ? ia + 1 : st.at[j].hi + e;
-      s_dw[group * p.d + ia] = da[j][e];
-      s_dw[group * p.d + ib] = db[j][e];
+      float a[2], b[2];
+      halves(da[j][e / 2], a[0], a[1]);
+      halves(db[j][e / 2], b[0], b[1]);
+      s_dw[group * p.d + ia] = a[e & 1];
+      s_dw[group * p.d + ib] = b[e & 1];
     }
   }
   __syncthreads();
@@ -500,7 +850,8 @@ murm_status check_args(const murm_norm_rope_args* a, bool backward) {
 // Widest run of elements (V) that every row, stride and unit boundary allows.
 int pick_v(const murm_norm_rope_args& a, bool backward) {
   const size_t es = elem_size(a.dtype);
-  for (int v = (int)(16 / es); v > 1; v = v == 8 ? 4 : 1) {
+  const int most = !a.normalize ? kRotV : backward ? kBwdV : kFwdV;
+  for (int v = (int)(16 / es) < most ? (int)(16 / es) : most; v > 1; v = v == 8 ? 4 : 1) {
     bool ok = a.rotary_dim % (2 * v) == 0 && (a.head_dim - a.rotary_dim) % (2 * v) == 0;
     for (const murm_head_rows* r : {&a.q, &a.k}) {
       if (r->heads == 0) continue;
@@ -518,14 +869,20 @@ int pick_v(const murm_norm_rope_args& a, bool backward) {
 
 Strides3 s3(const int64_t* s) { return Strides3{{s[0], s[1], s[2]}}; }
 
-// Heads per item of a tensor: all of them when the tokens alone give every SM `threads` threads
-// (the angles are then formed once per token), else as many as keep that many threads busy.
-int pick_chunk(int64_t tokens, int heads, int L, int threads, int step) {
-  const int64_t want = ((int64_t)kSms * threads / L + tokens - 1) / tokens;  // items per token
-  int64_t chunks = want < 1 ? 1 : want > heads ? heads : want;
-  int chunk = (int)((heads + chunks - 1) / chunks);
-  if (chunk > step) chunk = (chunk + step - 1) / step * step;
-  return chunk < heads ? chunk : heads;
+// Heads per item of a tensor, a multiple of `rows`: the fewest rounds of the resident groups over the
+// items, each as long as its heads and its angles.
+int pick_chunk(int64_t tokens, int heads, double groups, int rows) {
+  int best = rows;
+  double best_cost = 0;
+  for (int c = rows;; c += rows) {
+    const int64_t items = tokens * ((heads + c - 1) / c);
+    const double cost = std::ceil(items / groups) * (c + kAngleRows);
+    if (best_cost == 0 || cost < best_cost) {
+      best_cost = cost;
+      best = c;
+    }
+    if (c >= heads || c >= 64) return best;
+  }
 }
 
 void fill(const murm_norm_rope_args& a, int v, bool backward, Params* p) {
@@ -535,7 +892,6 @@ void fill(const murm_norm_rope_args& a, int v, bool backward, Params* p) {
   const int per_lane = v >= 4 ? 1 : 4;
   int L = 1;
   while (L * per_lane < p->units) L *= 2;
-  p->L = L;
   p->inverse = a.inverse ? 1 : 0;
   p->pos_type = a.position_type;
   p->eps = (float)a.eps;
@@ -563,8 +919,11 @@ void fill(const murm_norm_rope_args& a, int v, bool backward, Params* p) {
       for (int i = 0; i < pairs; ++i, f *= ratio) p->turns[i] = f;
     }
   }
-  const int groups = kThreads / L;
+  p->L = a.normalize ? L : (p->units + per_lane - 1) / per_lane;
+  const int groups = kThreads / p->L;
   const int64_t tokens = (int64_t)a.batch * a.tokens;
+  const int most = backward ? kBwdBlocks : kFwdBlocks;
+  const int rows = v < 4 ? 1 : !a.normalize ? kRotRows : backward ? kBwdRows : kFwdRows;
   const murm_head_rows* in[2] = {&a.q, &a.k};
   for (int t = 0; t < 2; ++t) {
     Rows& r = p->t[t];
@@ -577,20 +936,25 @@ void fill(const murm_norm_rope_args& a, int v, bool backward, Params* p) {
     r.w = s.weight;
     r.w_f32 = s.weight_dtype == MURM_F32;
     r.heads = s.heads;
-    r.chunk = pick_chunk(tokens, s.heads, L, 1024, backward ? 2 : kRowsInFlight);
-    r.items = (int)(tokens * ((s.heads + r.chunk - 1) / r.chunk));
+    r.chunk = pick_chunk(tokens, s.heads, (double)most * groups * s.heads / (a.q.heads + a.k.heads), rows);
+    r.chunks = (s.heads + r.chunk - 1) / r.chunk;
+    r.items = (int)(tokens * r.chunks);
     r.blocks = (r.items + groups - 1) / groups;
   }
-  if (backward) {  // at most kBwdBlocks blocks, shared out by heads
-    const int heads = a.q.heads + a.k.heads;
-    for (int t = 0; t < 2; ++t) {
-      Rows& r = p->t[t];
-      if (!r.heads) continue;
-      int cap = (int)((int64_t)kBwdBlocks * r.heads / heads);
-      if (cap < 1) cap = 1;
-      if (t == 1 && cap > kBwdBlocks - p->t[0].blocks) cap = kBwdBlocks - p->t[0].blocks;
-      if (r.blocks > cap) r.blocks = cap;
-    }
+  if (!a.normalize) return;
+  // no more blocks than are resident at once, shared out by work: an item's angles cost about as
+  // much as kAngleRows rows
+  double work[2] = {0, 0};
+  for (int t = 0; t < 2; ++t)
+    if (p->t[t].heads) work[t] = (double)p->t[t].items * (p->t[t].chunk + kAngleRows);
+  for (int t = 0; t < 2; ++t) {
+    Rows& r = p->t[t];
+    if (!r.heads) continue;
+    int cap = (int)(most * work[t] / (work[0] + work[1]));
+    if (cap < 1) cap = 1;
+    if (t == 1 && cap > most - p->t[0].blocks) cap = most - p->t[0].blocks;
+    if (t == 0 && cap == most && work[1] > 0) cap = most - 1;
+    if (r.blocks > cap) r.blocks = cap;
   }
 }
 
@@ -599,15 +963,24 @@ murm_status launch(const murm_norm_rope_args& a, bool backward, cudaStream_t st)
   Params p{};
   fill(a, V, backward, &p);
   const int blocks = p.t[0].blocks + p.t[1].blocks;
-  if (!backward) {
-    if (a.normalize) MURM_LAUNCH("norm_rope_fwd", (k_rope_fwd<T, V, INTER, true>), blocks, kThreads, 0, st, p);
-    else MURM_LAUNCH("rope_fwd", (k_rope_fwd<T, V, INTER, false>), blocks, kThreads, 0, st, p);
+  constexpr int U = UnitsPerLane<V>::v;
+  cudaError_t e = cudaSuccess;
+  if (!a.normalize) {
+    MURM_LAUNCH("rotate", (k_rotate<T, V, INTER>), blocks, kThreads, 0, st, p);
+  } else if (!backward) {
+    constexpr int smem = Ring<T, V, U, 1, kFwdDepth, U == 1 ? kFwdRows : 1>::kBytes;
+    auto* kernel = k_norm_rope_fwd<T, V, INTER>;
+    if (smem > 48 * 1024) e = smem_opt_in(kernel, smem);
+    if (e == cudaSuccess) MURM_LAUNCH("norm_rope_fwd", kernel, blocks, kThreads, smem, st, p);
   } else {
     const bool sums = a.q.grad_weight || a.k.grad_weight;
     p.part = sums ? static_cast<float*>(a.workspace) : nullptr;
-    const size_t smem = sums ? (size_t)(kThreads / p.L) * a.head_dim * sizeof(float) : 0;
-    MURM_LAUNCH("norm_rope_bwd", (k_norm_rope_bwd<T, V, INTER>), blocks, kThreads, smem, st, p);
-    if (sums) {
+    const int rings = Ring<T, V, U, 2, kBwdDepth, U == 1 ? kBwdRows : 1>::kBytes, dw = (kThreads / p.L) * a.head_dim * (int)sizeof(float);
+    const int smem = rings > dw ? rings : dw;
+    auto* kernel = k_norm_rope_bwd<T, V, INTER>;
+    if (smem > 48 * 1024) e = smem_opt_in(kernel, smem);
+    if (e == cudaSuccess) MURM_LAUNCH("norm_rope_bwd", kernel, blocks, kThreads, smem, st, p);
+    if (sums && e == cudaSuccess) {
       Finish f{};
       const murm_head_rows* in[2] = {&a.q, &a.k};
       for (int t = 0; t < 2; ++t) {
@@ -620,7 +993,7 @@ murm_status launch(const murm_norm_rope_args& a, bool backward, cudaStream_t st)
                   (const float*)p.part, a.head_dim, f);
     }
   }
-  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? MURM_OK : bad(MURM_ERR_CUDA, "norm_rope launch: %s", cudaGetErrorString(e));
 }
 
