@@ -271,7 +271,7 @@ __device__ __forceinline__ void activate_as(float (&v)[Out<T>::kCols], uint32_t 
     float d[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[j * kPer + i] = act_value<Out<T>::kFast>(v[j * kPer + i], ACT, d[i]);
-    if (SLOPE) sts128(buf + chunk_at(lane, j), pack16<T>(d));
+    if (SLOPE) sts128(buf + chunk_at(lane, j), pack16<Slope<T>>(d));
   }
 }
 template <typename T, bool SLOPE>
@@ -471,7 +471,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (p.slope) {
           buffer_free();
           activate<T, true>(v, p.act, sbuf, lane);
-          send(&map_slope, p.slope_tma, static_cast<T*>(p.slope), p.N, row, n, row);
+          send(&map_slope, p.slope_tma, static_cast<T*>(p.slope), p.N, row, n, row);  // by size alone
         } else {
           activate<T, false>(v, p.act, sbuf, lane);
         }
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(256)
     if (n + j >= p.N) break;
     if (p.bias) z[j] += Elem<T>::load(static_cast<const T*>(p.bias) + n + j);
     float slope, y = act_value<Out<T>::kFast>(z[j], p.act, slope);
-    if (p.slope) Elem<T>::store(static_cast<T*>(p.slope) + m * p.N + n + j, slope);
+    if (p.slope) Elem<Slope<T>>::store(static_cast<Slope<T>*>(p.slope) + m * p.N + n + j, slope);
     if (p.res) y += Elem<T>::load(static_cast<const T*>(p.res) + m * p.ldr + n + j);
     Elem<T>::store(static_cast<T*>(p.out) + m * p.ldo + n + j, y);
   }

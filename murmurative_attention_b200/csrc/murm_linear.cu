@@ -66,22 +66,23 @@ constexpr int kDzDepth = 4;
 
 template <typename T, int V, bool SLOPE>
 __global__ void __launch_bounds__(kDzThreads, 3)
-    k_dz(const T* dy, int64_t ldy, const T* slope, int M, int N, int cols, int chunk, Operand dz, float* part) {
+    k_dz(const T* dy, int64_t ldy, const Slope<T>* slope, int M, int N, int cols, int chunk, Operand dz, float* part) {
   __shared__ float s[kDzThreads * V];  // [row group][column]
   const int tx = threadIdx.x & (cols - 1), ty = threadIdx.x / cols, rows = kDzThreads / cols;
   const int n = (blockIdx.x * cols + tx) * V;
   const int m1 = (int)min((int64_t)M, (int64_t)(blockIdx.y + 1) * chunk);
   constexpr int kDepth = SLOPE ? kDzDepth : 2 * kDzDepth;
   using P = Pack<T, V>;
+  using PS = Pack<Slope<T>, V>;
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  auto row = [&](int r, const P& g, const P& sl) {
+  auto row = [&](int r, const P& g, const PS& sl) {
     float d[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       d[e] = Elem<T>::load(g.e + e);
-      if (SLOPE) d[e] *= Elem<T>::load(sl.e + e);
+      if (SLOPE) d[e] *= Elem<Slope<T>>::load(sl.e + e);
       acc[e] += d[e];
     }
     if (SLOPE && dz.p) store_operand<T, V>(dz, (int64_t)r * dz.ld + n, d);
@@ -89,13 +90,14 @@ __global__ void __launch_bounds__(kDzThreads, 3)
   if (n < N) {  // V divides N
     int m = blockIdx.y * chunk + ty;
     const T* pg = dy + (int64_t)m * ldy + n;
-    const T* ps = slope + (int64_t)m * N + n;
+    const Slope<T>* ps = slope + (int64_t)m * N + n;
     for (; m + (kDepth - 1) * rows < m1; m += kDepth * rows) {
-      P g[kDepth], sl[kDepth];
+      P g[kDepth];
+      PS sl[kDepth];
 #pragma unroll
       for (int i = 0; i < kDepth; ++i) {
         g[i] = *reinterpret_cast<const P*>(pg);
-        if (SLOPE) sl[i] = *reinterpret_cast<const P*>(ps);
+        if (SLOPE) sl[i] = *reinterpret_cast<const PS*>(ps);
         pg += (int64_t)rows * ldy;
         ps += (int64_t)rows * N;
       }
@@ -104,8 +106,8 @@ __global__ void __launch_bounds__(kDzThreads, 3)
     }
     for (; m < m1; m += rows) {
       const P g = *reinterpret_cast<const P*>(pg);
-      P sl{};
-      if (SLOPE) sl = *reinterpret_cast<const P*>(ps);
+      PS sl{};
+      if (SLOPE) sl = *reinterpret_cast<const PS*>(ps);
       row(m, g, sl);
       pg += (int64_t)rows * ldy;
       ps += (int64_t)rows * N;
@@ -156,10 +158,10 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
   const T* dy = static_cast<const T*>(a.grad_out);
   if (a.activation == MURM_ACT_NONE)
     MURM_LAUNCH("linear_col_part", (k_dz<T, V, false>), grid, kDzThreads, 0, st, dy, a.go_stride,
-                (const T*)nullptr, M, N, cols, chunk, dz, part);
+                (const Slope<T>*)nullptr, M, N, cols, chunk, dz, part);
   else
     MURM_LAUNCH("linear_dz", (k_dz<T, V, true>), grid, kDzThreads, 0, st, dy, a.go_stride,
-                static_cast<const T*>(a.slope), M, N, cols, chunk, dz, part);
+                static_cast<const Slope<T>*>(a.slope), M, N, cols, chunk, dz, part);
   if (part)
     MURM_LAUNCH("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 256, 0, st, (const float*)part, chunks, N,
                 static_cast<T*>(a.grad_bias));

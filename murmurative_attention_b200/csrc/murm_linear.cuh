@@ -25,11 +25,17 @@ struct Gemm {
   const void* bias;
   const void* res; int64_t ldr;
   void* out; int64_t ldo;
-  void* slope;   // [M][N] contiguous: act'(z), or NULL
+  void* slope;   // [M][N] contiguous: act'(z) as Slope<T>, or NULL
   int act;       // murm_activation
 };
 size_t gemm_workspace(const Gemm& g);
 murm_status gemm(const Gemm& g, void* workspace, cudaStream_t st);
+
+// Type of the saved slopes: fp16 beside 16-bit tensors (slopes are of order one, so it holds them
+// eight times nearer than bf16 would), fp32 beside fp32.
+template <typename T> struct SlopeOf { using type = __half; };
+template <> struct SlopeOf<float> { using type = float; };
+template <typename T> using Slope = typename SlopeOf<T>::type;
 
 // Packing of a row-major matrix into an Operand: fp32 always (three planes), 16-bit data when its
 // address or stride is not one TMA can take.
