@@ -350,6 +350,7 @@ BwdPlan plan_bwd(const murm_linear_bwd_args& a) {
 }
 
 murm_status run_fwd(const murm_linear_args& a, cudaStream_t st) {
+  if (few_rows(a)) return few_rows_forward(a, st);
   const FwdPlan p = plan_fwd(a);
   if (murm_status s = check_ws(a.workspace, a.workspace_bytes, p.l.bytes)) return s;
   if (murm_status s = fill(p.x, p.l, st)) return s;
@@ -400,7 +401,7 @@ extern "C" {
 murm_status murm_linear_workspace(const murm_linear_args* args, size_t* bytes) {
   if (!bytes) return bad(MURM_ERR_INVALID_ARGUMENT, "bytes is NULL");
   if (murm_status s = check_fwd(args)) return s;
-  *bytes = args->rows ? plan_fwd(*args).l.bytes : 0;
+  *bytes = args->rows && !few_rows(*args) ? plan_fwd(*args).l.bytes : 0;
   return MURM_OK;
 }
 murm_status murm_linear_fwd(const murm_linear_args* args, void* stream) {

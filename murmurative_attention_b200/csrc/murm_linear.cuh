@@ -37,6 +37,10 @@ template <typename T> struct SlopeOf { using type = __half; };
 template <> struct SlopeOf<float> { using type = float; };
 template <typename T> using Slope = typename SlopeOf<T>::type;
 
+// The forward for a few rows (murm_linear_rows.cu), where it takes the call: no workspace.
+bool few_rows(const murm_linear_args& a);
+murm_status few_rows_forward(const murm_linear_args& a, cudaStream_t st);
+
 // Packing of a row-major matrix into an Operand: fp32 always (three planes), 16-bit data when its
 // address or stride is not one TMA can take.
 struct Matrix {
