@@ -70,8 +70,23 @@ struct Args {
   const void* res; int64_t ldr; int res_vec;
   void* out; int64_t ldo; int out_tma;
   void* slope; int slope_tma;
-  int split_rows;  // rows of one split's partial result
+  int partial;     // out: fp32 sums of K splits, tiles side by side, splits `split_rows` rows apart
+  int split_rows;
 };
+struct Problem {
+  CUtensorMap a, b, out, slope;
+  Args p;
+};
+// One launch: the items of one or two products. Pair j takes the positions j, j + pairs, ...; with
+// `tabled` a position's item is order[position] (kNone: nothing).
+constexpr int kMaxOrder = 8 * kPairs;
+constexpr uint16_t kNone = 0xffff;
+struct Launch {
+  Problem q[2];
+  int items, positions, tabled;
+  uint16_t order[kMaxOrder];
+};
+static_assert(sizeof(Launch) <= 4000, "kernel parameters");
 
 // Plane pairs of an fp32 product, smallest terms first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0).
 __device__ __forceinline__ int plane_a(int pair) { return (0x021010 >> (4 * (5 - pair))) & 15; }
@@ -289,14 +304,21 @@ __device__ __forceinline__ void activate(float (&v)[Out<T>::kCols], int act, uin
 // the product
 // ---------------------------------------------------------------------------
 struct Item {
+  int which;  // the product; -1: nothing at this position
   int m0, n0, split, i0, i1;
 };
 // Tiles run down kGroupM tile rows before the next tile column, so that the tiles in flight at once
 // read few rows of A and few of B from L2.
 constexpr int kGroupM = 8;
-template <int BN>
-__device__ __forceinline__ Item item_at(const Args& p, int item) {
+template <int BN, bool TWO>
+__device__ __forceinline__ Item item_at(const Launch& l, int position) {
   Item r;
+  int item = TWO && l.tabled ? l.order[position] : position;
+  r.which = -1;
+  if (item >= l.items) return r;
+  r.which = TWO && item >= l.q[0].p.items;
+  const Args& p = l.q[TWO ? r.which : 0].p;
+  if (TWO && r.which) item -= l.q[0].p.items;
   r.split = item / p.tiles;
   const int t = item - r.split * p.tiles;
   const int g = t / (kGroupM * p.tiles_n), in = t - g * kGroupM * p.tiles_n;
@@ -309,11 +331,12 @@ __device__ __forceinline__ Item item_at(const Args& p, int item) {
   return r;
 }
 
-template <typename T, int BN>
+// TWO: a launch of two products, whose epilogues only store. With one, its parameters are at fixed
+// places; with two, what the loops need of them is read once per item (read by a computed place in
+// every round they cost a fifth of the time).
+template <typename T, int BN, bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    k_gemm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-              const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_slope,
-              const __grid_constant__ Args p) {
+    k_gemm_tc(const __grid_constant__ Launch l) {
   using L = Tile<BN>;
   constexpr int kCols = Out<T>::kCols;
   extern __shared__ uint8_t raw[];
@@ -349,32 +372,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint32_t s = 0, ph = 0;  // stage and its round's parity
     int issued = 0;
     bool ok = true;
-    for (int item = first; ok && item < p.items; item += step) {
-      const Item t = item_at<BN>(p, item);
+    for (int at = first; ok && at < l.positions; at += step) {
+      const Item t = item_at<BN, TWO>(l, at);
+      if (t.which < 0) continue;
+      const Problem& pr = l.q[TWO ? t.which : 0];
+      const CUtensorMap *map_a = &pr.a, *map_b = &pr.b;
+      const int a_mn = pr.p.a_mn, b_mn = pr.p.b_mn, fp32 = pr.p.fp32, kblocks = pr.p.kblocks;
       const int ma = t.m0 + (int)rank * 128, nb = t.n0 + (int)rank * (BN / 2);
-      int pair = p.fp32 ? t.i0 / p.kblocks : 0;
-      int kb = t.i0 - pair * p.kblocks;
+      int pair = fp32 ? t.i0 / kblocks : 0;
+      int kb = t.i0 - pair * kblocks;
       for (int i = t.i0; i < t.i1; ++i) {
         if (!(ok = wait(&bars->empty[s], ph ^ 1))) break;
         if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
         const uint32_t bar = map_to_first(&bars->full[s]);
         const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
         const int k = kb * kBK;
-        const int pa = p.fp32 ? plane_a(pair) : 0, pb = p.fp32 ? plane_b(pair) : 0;
-        if (p.a_mn) {
-          tma_load_pair(sa, &map_a, ma, k, pa, bar);
-          tma_load_pair(sa + 8192, &map_a, ma + 64, k, pa, bar);
+        const int pa = fp32 ? plane_a(pair) : 0, pb = fp32 ? plane_b(pair) : 0;
+        if (a_mn) {
+          tma_load_pair(sa, map_a, ma, k, pa, bar);
+          tma_load_pair(sa + 8192, map_a, ma + 64, k, pa, bar);
         } else {
-          tma_load_pair(sa, &map_a, k, ma, pa, bar);
+          tma_load_pair(sa, map_a, k, ma, pa, bar);
         }
-        if (p.b_mn) {
+        if (b_mn) {
 #pragma unroll
-          for (int c = 0; c < BN / 128; ++c) tma_load_pair(sb + c * 8192, &map_b, nb + c * 64, k, pb, bar);
+          for (int c = 0; c < BN / 128; ++c) tma_load_pair(sb + c * 8192, map_b, nb + c * 64, k, pb, bar);
         } else {
-          tma_load_pair(sb, &map_b, k, nb, pb, bar);
+          tma_load_pair(sb, map_b, k, nb, pb, bar);
         }
         ++issued;
-        if (++kb == p.kblocks) { kb = 0; ++pair; }
+        if (++kb == kblocks) { kb = 0; ++pair; }
         if (++s == L::kStages) { s = 0; ph ^= 1; }
       }
     }
@@ -389,15 +416,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // Operand descriptors: K-major steps through 16 of a row's 64 elements (32 bytes), MN-major
     // through 16 of 64 rows (2 KB), its 64-wide column blocks 8 KB apart. Only the low word, which
     // holds the address, changes.
-    const uint64_t da = smem_desc(sbase, p.a_mn ? 8192 : 16, 1024, kSwizzle128B);
-    const uint64_t db = smem_desc(sbase + kABytes, p.b_mn ? 8192 : 16, 1024, kSwizzle128B);
-    const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
-    const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
     uint32_t s = 0, ph = 0;
     int t = 0;
     bool ok = true;
-    for (int item = first; ok && item < p.items; item += step, ++t) {
-      const Item w = item_at<BN>(p, item);
+    for (int at = first; ok && at < l.positions; at += step) {
+      const Item w = item_at<BN, TWO>(l, at);
+      if (w.which < 0) continue;
+      const Args& p = l.q[TWO ? w.which : 0].p;
+      const uint64_t da = smem_desc(sbase, p.a_mn ? 8192 : 16, 1024, kSwizzle128B);
+      const uint64_t db = smem_desc(sbase + kABytes, p.b_mn ? 8192 : 16, 1024, kSwizzle128B);
+      const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
+      const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4, idesc = p.idesc;
       const int buf = t & 1;
       if (!(ok = wait(&bars->acc_free[buf], ((t >> 1) & 1) ^ 1))) break;
       tc_fence_after();
@@ -409,7 +438,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t a_lo = (uint32_t)da + s * (L::kStage >> 4), b_lo = (uint32_t)db + s * (L::kStage >> 4);
 #pragma unroll
         for (int kk = 0; kk < kBK / 16; ++kk) {
-          mma_pair(d, ((uint64_t)a_hi << 32) | a_lo, ((uint64_t)b_hi << 32) | b_lo, p.idesc, more);
+          mma_pair(d, ((uint64_t)a_hi << 32) | a_lo, ((uint64_t)b_hi << 32) | b_lo, idesc, more);
           a_lo += a_step;
           b_lo += b_step;
           more = 1;
@@ -418,6 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (++s == L::kStages) { s = 0; ph ^= 1; }
       }
       if (ok) commit_pair(&bars->acc_full[buf]);
+      ++t;
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
@@ -427,33 +457,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int t = 0;
     bool ok = true;
     // sends the buffer's rows out, once every lane has written its own
-    auto send = [&](const CUtensorMap* map, int tma, T* base, int64_t ld, int row, int n, int store_row) {
+    auto send = [&](const CUtensorMap* map, int tma, T* base, int64_t ld, int row, int n, int store_row, int M, int N) {
       if (tma) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tma_store_2d(map, sbuf, n, store_row);
       } else {
         __syncwarp();
-        copy_rows<T, true>(pbuf, base + (int64_t)row * ld + n, ld, min(32, p.M - row), p.N - n, lane);
+        copy_rows<T, true>(pbuf, base + (int64_t)row * ld + n, ld, min(32, M - row), N - n, lane);
       }
     };
     auto buffer_free = [&]() {  // its last store, or the warp's own copies, have read it
       if (lane == 0) tma_store_wait_read();
       __syncwarp();
     };
-    for (int item = first; ok && item < p.items; item += step, ++t) {
-      const Item it = item_at<BN>(p, item);
+    for (int at = first; ok && at < l.positions; at += step) {
+      const Item it = item_at<BN, TWO>(l, at);
+      if (it.which < 0) continue;
+      const Problem& pr = l.q[TWO ? it.which : 0];
+      const Args& p = pr.p;
+      const CUtensorMap* map_out = &pr.out;
+      const int M = p.M, N = p.N, out_tma = p.out_tma, partial = p.partial, split_row = it.split * p.split_rows;
       const int buf = t & 1;
       const int row = it.m0 + (int)rank * 128 + w * 32;
       const int n_first = it.n0 + quarter * (BN / 4);
-      const int n_end = row < p.M ? min(p.N, n_first + BN / 4) : 0;
-      const T* res = static_cast<const T*>(p.res) + (int64_t)row * p.ldr;
-      const bool res_vec = p.res && p.res_vec;
+      const int n_end = row < M ? min(N, n_first + BN / 4) : 0;
+      const T* res = TWO ? nullptr : static_cast<const T*>(p.res) + (int64_t)row * p.ldr;
+      const bool res_vec = !TWO && p.res && p.res_vec;
       uint4 rv[4], bv[4];
       if (res_vec && n_first < n_end)
-        load_rows(res + n_first, p.ldr, p.M - row, p.N - n_first, lane, rv);
-      if (p.bias_vec && n_first < n_end) load_bias(static_cast<const T*>(p.bias) + n_first, p.N - n_first, bv);
+        load_rows(res + n_first, p.ldr, M - row, N - n_first, lane, rv);
+      if (!TWO && p.bias_vec && n_first < n_end) load_bias(static_cast<const T*>(p.bias) + n_first, N - n_first, bv);
       ok = wait(&bars->acc_full[buf], (t >> 1) & 1);
+      ++t;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -463,32 +499,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if constexpr (kCols == 32) tmem_ld32(acc + (n - n_first), v);
         else tmem_ld16(acc + (n - n_first), v);
         tmem_wait_ld();
-        if (p.bias) {
-          add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, bv, p.N - n, v);
-          if (p.bias_vec && n + kCols < n_end)
-            load_bias(static_cast<const T*>(p.bias) + n + kCols, p.N - n - kCols, bv);
+        if constexpr (sizeof(T) == 2) {
+          if (partial) {  // 32 columns of fp32: two rows' worth of the buffer
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              buffer_free();
+              write_row<float>(sbuf, lane, *reinterpret_cast<const float(*)[16]>(v + 16 * h));
+              send(map_out, 1, static_cast<T*>(nullptr), 0, row, n + 16 * h, split_row + row, M, N);
+            }
+            continue;
+          }
         }
-        if (p.slope) {
+        if (!TWO && p.bias) {
+          add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, bv, N - n, v);
+          if (p.bias_vec && n + kCols < n_end)
+            load_bias(static_cast<const T*>(p.bias) + n + kCols, N - n - kCols, bv);
+        }
+        if (!TWO && p.slope) {
           buffer_free();
           activate<T, true>(v, p.act, sbuf, lane);
-          send(&map_slope, p.slope_tma, static_cast<T*>(p.slope), p.N, row, n, row);  // by size alone
-        } else {
+          send(&pr.slope, p.slope_tma, static_cast<T*>(p.slope), N, row, n, row, M, N);  // by size alone
+        } else if (!TWO) {
           activate<T, false>(v, p.act, sbuf, lane);
         }
         buffer_free();
-        if (p.res) {
+        if (!TWO && p.res) {
           if (res_vec) {
             put_rows(sbuf, lane, rv);
             if (n + kCols < n_end)
-              load_rows(res + n + kCols, p.ldr, p.M - row, p.N - n - kCols, lane, rv);
+              load_rows(res + n + kCols, p.ldr, M - row, N - n - kCols, lane, rv);
           } else {
-            copy_rows<T, false>(pbuf, const_cast<T*>(res) + n, p.ldr, min(32, p.M - row), p.N - n, lane);
+            copy_rows<T, false>(pbuf, const_cast<T*>(res) + n, p.ldr, min(32, M - row), N - n, lane);
           }
           __syncwarp();
           add_row<T>(sbuf, lane, v);
         }
         write_row<T>(sbuf, lane, v);
-        send(&map_out, p.out_tma, static_cast<T*>(p.out), p.ldo, row, n, it.split * p.split_rows + row);
+        send(map_out, out_tma, static_cast<T*>(p.out), p.ldo, row, n, split_row + row, M, N);
       }
       tc_fence_before();
       __syncwarp();
@@ -584,6 +631,13 @@ struct Config {
   int bn, splits, iters, total, kblocks, tiles_m, tiles_n;
 };
 
+Config config(const Gemm& g, int bn, int splits) {
+  const int kblocks = (g.K + kBK - 1) / kBK;
+  const int total = kblocks * (g.a.planes == 3 ? 6 : 1);
+  const int iters = (total + splits - 1) / splits;
+  return Config{bn, (total + iters - 1) / iters, iters, total, kblocks, (g.M + 255) / 256, (g.N + bn - 1) / bn};
+}
+
 // Tile width and K splits by estimated time, in microseconds measured on B200:
 // - a 64-deep stage takes 0.35 of a 256-wide tile (its 64 KB per CTA pair are about what L2 delivers
 //   to two SMs in that time, which is also the MMAs' own) and 0.31 of a 128-wide one, bound by the
@@ -591,29 +645,108 @@ struct Config {
 //   leaves fewer rounds: 512 x 1024 x 1024: 9.5 us at 128, 10.2 at 256; 8192 x 1024 x 1024: 27.5 and 18.1.
 // - a split costs a second launch, and its fp32 sums about 4.8 MB per us:
 //   1024 x 1024 x 8192 (dW): 50 us in one part, 24 in four, 28 in eight.
-Config choose(const Gemm& g) {
-  Config best{};
+// - a launch of its own costs about 5 (prologue, first loads, last epilogue).
+constexpr double kLaunchUs = 5.0;
+double stage_us(const Gemm& g, int bn) { return (bn == 256 ? 0.35 : 0.31) * (g.a_mn ? 1.15 : 1.0); }
+double split_us(const Config& c) {
+  return c.splits == 1 ? 0.0 : 4.0 + (double)c.tiles_m * c.tiles_n * 256 * c.bn * 4 * c.splits / 4.8e6;
+}
+bool split_fits(const Config& c, int splits) {
+  return splits == 1 || (c.total / splits >= 2 && (int64_t)c.tiles_m * c.tiles_n * splits <= 2 * kPairs);
+}
+double choose_one(const Gemm& g, Config* best) {
   double best_t = 0;
-  const int kblocks = (g.K + kBK - 1) / kBK;
-  const int total = kblocks * (g.a.planes == 3 ? 6 : 1);
-  for (int bn : {256, 128}) {
-    const int tm = (g.M + 255) / 256, tn = (g.N + bn - 1) / bn;
-    const int64_t tiles = (int64_t)tm * tn;
-    const double stage = (bn == 256 ? 0.35 : 0.31) * (g.a_mn ? 1.15 : 1.0);
+  for (int bn : {256, 128})
     for (int splits = 1; splits <= 16; ++splits) {
-      if (splits > 1 && (total / splits < 2 || tiles * splits > 2 * kPairs)) break;
-      const int iters = (total + splits - 1) / splits;
-      const int used = (total + iters - 1) / iters;
-      const int64_t rounds = (tiles * used + kPairs - 1) / kPairs;
-      double t = rounds * iters * stage;
-      if (used > 1) t += 4.0 + (double)tiles * 256 * bn * 4 * used / 4.8e6;
+      const Config c = config(g, bn, splits);
+      if (!split_fits(c, splits)) break;
+      const int64_t rounds = ((int64_t)c.tiles_m * c.tiles_n * c.splits + kPairs - 1) / kPairs;
+      const double t = rounds * c.iters * stage_us(g, bn) + split_us(c);
       if (best_t == 0 || t < best_t) {
         best_t = t;
-        best = Config{bn, used, iters, total, kblocks, tm, tn};
+        *best = c;
       }
     }
+  return best_t + kLaunchUs;
+}
+
+struct Plan {
+  Config c[2];
+  bool together;
+};
+// Two products together: no shorter than their work over all pairs, than the longest item, or than
+// what the last item of a pair leaves idle; side by side they also run a tenth slower than alone (two
+// sets of operands in L2, and no SM left idle whose power the others could use). It pays for short
+// products: both gradients of 8192 x 1024 x 1024 41.6 us, apart 45.6; of 32768 x 1024 x 4096 428 and 407.
+constexpr double kTogether = 1.1;
+Plan choose(const Gemm* g, int count) {
+  Plan p{};
+  double apart = 0;
+  for (int i = 0; i < count; ++i) apart += choose_one(g[i], &p.c[i]);
+  if (count < 2) return p;
+  constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+  struct Option {
+    Config c;
+    double item, work, extra;
+  } opt[2][8];
+  for (int bn : {256, 128}) {
+    int n[2] = {0, 0};
+    for (int i = 0; i < 2; ++i)
+      for (int splits : kSplits) {
+        Option& o = opt[i][n[i]];
+        o.c = config(g[i], bn, splits);
+        if (!split_fits(o.c, splits)) break;
+        o.item = o.c.iters * stage_us(g[i], bn);
+        o.work = o.item * o.c.tiles_m * o.c.tiles_n * o.c.splits;
+        o.extra = split_us(o.c);
+        ++n[i];
+      }
+    for (int a = 0; a < n[0]; ++a)
+      for (int b = 0; b < n[1]; ++b) {
+        const Option &x = opt[0][a], &y = opt[1][b];
+        const double work = kTogether * (x.work + y.work) / kPairs + (x.item < y.item ? x.item : y.item) / 2;
+        const double longest = x.item > y.item ? x.item : y.item;
+        const double t = kLaunchUs + x.extra + y.extra + (work > longest ? work : longest);
+        if (t < apart) {
+          apart = t;
+          p.c[0] = x.c;
+          p.c[1] = y.c;
+          p.together = true;
+        }
+      }
   }
-  return best;
+  return p;
+}
+
+// The items of both products over the pairs, the longer ones (the first n0) first, then the others to
+// the pairs with the least to do so far. All items of a product are taken to be of one length, so the
+// pairs are of two kinds at any time: those with one more of the long items and the rest.
+void fill_order(Launch* l, int n0, int len0, int n1, int len1, int pairs) {
+  for (int i = 0; i < kMaxOrder; ++i) l->order[i] = kNone;
+  int slot[2] = {n0 / pairs + (n0 % pairs ? 1 : 0), n0 / pairs};  // rows of the table taken, per kind
+  const int cut = n0 % pairs;                                     // pairs below it have one more
+  for (int i = 0; i < n0; ++i) l->order[i] = (uint16_t)i;
+  int load[2] = {slot[0] * len0, slot[1] * len0};
+  int next = n0;
+  const int end = n0 + n1;
+  while (next < end) {
+    const int kind = cut && load[0] < load[1] ? 0 : 1;
+    const int from = kind ? cut : 0, to = kind ? pairs : cut;
+    for (int j = from; j < to && next < end; ++j) {
+      const int at = slot[kind] * pairs + j;
+      if (at >= kMaxOrder) {  // too uneven for the table: in plain order
+        l->tabled = 0;
+        l->positions = l->items;
+        return;
+      }
+      l->order[at] = (uint16_t)next++;
+    }
+    ++slot[kind];
+    load[kind] += len1;
+  }
+  const int rows = slot[0] > slot[1] ? slot[0] : slot[1];
+  l->tabled = 1;
+  l->positions = rows * pairs;
 }
 
 // Operands: three dimensions (the planes) and 128-byte swizzled rows; results (planes = 0): two
@@ -641,48 +774,13 @@ void launch(const char* name, void (*kernel)(KArgs...), dim3 grid, int threads, 
   MURM_LAUNCH_PDL(name, kernel, grid, threads, smem, st, args...);
 }
 
+// Fills a launch's product.
 template <typename T, int BN>
-murm_status launch_tc(const Gemm& g, const Config& c, Args p, void* out, int64_t ldo, int64_t out_rows, int64_t out_cols,
-                      cudaStream_t st) {
+CUresult describe(const Gemm& g, const Config& c, void* workspace, Problem* q) {
   const size_t es = sizeof(T);
   constexpr int kCols = Out<T>::kCols;
-  const CUtensorMapDataType op = g.dtype == MURM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUtensorMapDataType ot = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(g.dtype);
-  CUtensorMap ma, mb, mo{}, ms{};
-  CUresult r;
-  if (g.a_mn) r = encode(&ma, op, 2, g.a.p, g.M, g.K, g.a.ld, g.a.planes, g.a.plane, 64, 64);
-  else r = encode(&ma, op, 2, g.a.p, g.K, g.M, g.a.ld, g.a.planes, g.a.plane, 64, 128);
-  if (r == CUDA_SUCCESS) {
-    if (g.b_mn) r = encode(&mb, op, 2, g.b.p, g.N, g.K, g.b.ld, g.b.planes, g.b.plane, 64, 64);
-    else r = encode(&mb, op, 2, g.b.p, g.K, g.N, g.b.ld, g.b.planes, g.b.plane, 64, BN / 2);
-  }
-  p.out = out;
-  p.ldo = ldo;
-  p.out_tma = tma_rows(out, ldo, es);
-  if (r == CUDA_SUCCESS && p.out_tma) r = encode(&mo, ot, es, out, out_cols, out_rows, ldo, 0, 0, kCols, 32);
-  const int per = 16 / (int)es;
-  p.res_vec = p.res && tma_rows(p.res, p.ldr, es) && g.N % per == 0;
-  p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && g.N % per == 0;
-  if (p.slope) {
-    p.slope_tma = tma_rows(p.slope, g.N, es);
-    if (r == CUDA_SUCCESS && p.slope_tma) r = encode(&ms, ot, es, p.slope, g.N, g.M, g.N, 0, 0, kCols, 32);
-  }
-  if (r != CUDA_SUCCESS) {
-    char msg[96];
-    snprintf(msg, sizeof msg, "linear: a tensor map was refused (%d)", (int)r);
-    return report_error(MURM_ERR_CUDA, msg);
-  }
-  const int items = p.items;
-  const int grid = 2 * (items < kPairs ? items : kPairs);
-  if (cudaError_t e = smem_opt_in(k_gemm_tc<T, BN>, Tile<BN>::kSmem))
-    return report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
-  launch("linear_gemm", k_gemm_tc<T, BN>, dim3(grid), kThreads, Tile<BN>::kSmem, st, ma, mb, mo, ms, p);
-  return MURM_OK;
-}
-
-template <typename T>
-murm_status run(const Gemm& g, const Config& c, void* workspace, cudaStream_t st) {
-  Args p{};
+  Args& p = q->p;
+  p = Args{};
   p.M = g.M; p.N = g.N;
   p.kblocks = c.kblocks; p.iters = c.iters; p.total = c.total; p.splits = c.splits;
   p.tiles_m = c.tiles_m;
@@ -692,50 +790,116 @@ murm_status run(const Gemm& g, const Config& c, void* workspace, cudaStream_t st
   p.idesc = idesc_f16(g.dtype == MURM_F16 ? 0 : 1, 256, c.bn, g.a_mn, g.b_mn);
   p.a_mn = g.a_mn; p.b_mn = g.b_mn;
   p.fp32 = g.a.planes == 3;
+  const CUtensorMapDataType op = g.dtype == MURM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapDataType ot = map_type(g.dtype);
+  CUresult r;
+  if (g.a_mn) r = encode(&q->a, op, 2, g.a.p, g.M, g.K, g.a.ld, g.a.planes, g.a.plane, 64, 64);
+  else r = encode(&q->a, op, 2, g.a.p, g.K, g.M, g.a.ld, g.a.planes, g.a.plane, 64, 128);
+  if (r != CUDA_SUCCESS) return r;
+  if (g.b_mn) r = encode(&q->b, op, 2, g.b.p, g.N, g.K, g.b.ld, g.b.planes, g.b.plane, 64, 64);
+  else r = encode(&q->b, op, 2, g.b.p, g.K, g.N, g.b.ld, g.b.planes, g.b.plane, 64, BN / 2);
+  if (r != CUDA_SUCCESS) return r;
+  if (c.splits > 1) {  // partial sums alone; the epilogue follows in k_split_sum
+    p.partial = 1;
+    p.M = p.split_rows = c.tiles_m * 256;
+    p.N = c.tiles_n * BN;
+    p.out = workspace;
+    p.ldo = p.N;
+    p.out_tma = 1;
+    return encode(&q->out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, workspace, p.N, (int64_t)p.M * c.splits, p.ldo, 0, 0, 16,
+                  32);
+  }
   p.bias = g.bias; p.act = g.act;
   p.res = g.res; p.ldr = g.ldr;
+  p.out = g.out; p.ldo = g.ldo;
   p.slope = g.slope;
-  murm_status s;
-  if (c.splits == 1) {
-    s = c.bn == 256 ? launch_tc<T, 256>(g, c, p, g.out, g.ldo, g.M, g.N, st)
-                    : launch_tc<T, 128>(g, c, p, g.out, g.ldo, g.M, g.N, st);
-  } else {
-    Args q = p;  // partial sums alone
-    q.bias = q.res = nullptr;
-    q.slope = nullptr;
-    q.act = MURM_ACT_NONE;
-    const int rows = c.tiles_m * 256, cols = c.tiles_n * c.bn;
-    q.M = rows;
-    q.N = cols;
-    q.split_rows = rows;
-    s = c.bn == 256 ? launch_tc<float, 256>(g, c, q, workspace, cols, (int64_t)rows * c.splits, cols, st)
-                    : launch_tc<float, 128>(g, c, q, workspace, cols, (int64_t)rows * c.splits, cols, st);
-    if (s == MURM_OK) {
-      p.out = g.out;
-      p.ldo = g.ldo;
-      launch("linear_split_sum", k_split_sum<T>, dim3((g.N + 255) / 256, (g.M + 3) / 4), 256, 0, st,
-             static_cast<const float*>(workspace), (int64_t)rows * cols, cols, p);
-    }
+  const int per = 16 / (int)es;
+  p.res_vec = p.res && tma_rows(p.res, p.ldr, es) && g.N % per == 0;
+  p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && g.N % per == 0;
+  p.out_tma = tma_rows(g.out, g.ldo, es);
+  if (p.out_tma) r = encode(&q->out, ot, es, g.out, g.N, g.M, g.ldo, 0, 0, kCols, 32);
+  if (r == CUDA_SUCCESS && p.slope) {
+    p.slope_tma = tma_rows(p.slope, g.N, es);
+    if (p.slope_tma) r = encode(&q->slope, ot, es, p.slope, g.N, g.M, g.N, 0, 0, kCols, 32);
   }
-  if (s != MURM_OK) return s;
+  return r;
+}
+
+size_t split_bytes(const Config& c) {
+  return c.splits == 1 ? 0 : (size_t)c.splits * c.tiles_m * 256 * c.tiles_n * c.bn * sizeof(float);
+}
+
+// One launch of one or two products with the same tile width, then the sums of those with splits.
+template <typename T, int BN>
+murm_status launch_tc(const Gemm* g, const Config* c, int count, char* workspace, cudaStream_t st) {
+  Launch l;
+  l.items = l.tabled = 0;
+  // the product with the longer items comes first
+  const int swap = count == 2 && c[1].iters > c[0].iters;
+  float* part[2];
+  for (int i = 0; i < count; ++i) {
+    part[i] = reinterpret_cast<float*>(workspace);
+    workspace += split_bytes(c[i]);
+    const CUresult r = describe<T, BN>(g[i], c[i], part[i], &l.q[i ^ swap]);
+    if (r != CUDA_SUCCESS) {
+      char msg[96];
+      snprintf(msg, sizeof msg, "linear: a tensor map was refused (%d)", (int)r);
+      return report_error(MURM_ERR_CUDA, msg);
+    }
+    l.items += l.q[i ^ swap].p.items;
+  }
+  l.positions = l.items;
+  const int pairs = l.items < kPairs ? l.items : kPairs;
+  if (count == 2 && l.items <= kMaxOrder)
+    fill_order(&l, l.q[0].p.items, l.q[0].p.iters, l.q[1].p.items, l.q[1].p.iters, pairs);
+  auto* kernel = count == 2 ? k_gemm_tc<T, BN, true> : k_gemm_tc<T, BN, false>;
+  if (cudaError_t e = smem_opt_in(kernel, Tile<BN>::kSmem)) return report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
+  launch("linear_gemm", kernel, dim3(2 * pairs), kThreads, Tile<BN>::kSmem, st, l);
+  for (int i = 0; i < count; ++i) {
+    if (c[i].splits == 1) continue;
+    Args p = l.q[i ^ swap].p;
+    const int ldp = p.N;
+    const int64_t stride = (int64_t)p.M * p.N;
+    p.M = g[i].M; p.N = g[i].N;
+    p.bias = g[i].bias; p.act = g[i].act;
+    p.res = g[i].res; p.ldr = g[i].ldr;
+    p.out = g[i].out; p.ldo = g[i].ldo;
+    p.slope = g[i].slope;
+    launch("linear_split_sum", k_split_sum<T>, dim3((p.N + 255) / 256, (p.M + 3) / 4), 256, 0, st,
+           const_cast<const float*>(part[i]), stride, ldp, p);
+  }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MURM_OK : report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
 }
 
-}  // namespace
-
-size_t gemm_workspace(const Gemm& g) {
-  const Config c = choose(g);
-  return c.splits == 1 ? 0 : (size_t)c.splits * c.tiles_m * 256 * c.tiles_n * c.bn * sizeof(float);
+template <typename T>
+murm_status run(const Gemm* g, int count, char* workspace, cudaStream_t st) {
+  const Plan p = choose(g, count);
+  auto go = [&](const Gemm* gs, const Config* cs, int n, char* ws) {
+    return cs[0].bn == 256 ? launch_tc<T, 256>(gs, cs, n, ws, st) : launch_tc<T, 128>(gs, cs, n, ws, st);
+  };
+  if (p.together) return go(g, p.c, 2, workspace);
+  for (int i = 0; i < count; ++i) {
+    if (murm_status s = go(g + i, p.c + i, 1, workspace)) return s;
+    workspace += split_bytes(p.c[i]);
+  }
+  return MURM_OK;
 }
 
-murm_status gemm(const Gemm& g, void* workspace, cudaStream_t st) {
+}  // namespace
+
+size_t gemm_workspace(const Gemm* g, int count) {
+  const Plan p = choose(g, count);
+  return split_bytes(p.c[0]) + (count > 1 ? split_bytes(p.c[1]) : 0);
+}
+
+murm_status gemm(const Gemm* g, int count, void* workspace, cudaStream_t st) {
   if (!tc_tensor_map_encoder()) return report_error(MURM_ERR_CUDA, "linear: cuTensorMapEncodeTiled is not available");
-  const Config c = choose(g);
-  switch (g.dtype) {
-    case MURM_F32: return run<float>(g, c, workspace, st);
-    case MURM_F16: return run<__half>(g, c, workspace, st);
-    default: return run<__nv_bfloat16>(g, c, workspace, st);
+  char* ws = static_cast<char*>(workspace);
+  switch (g[0].dtype) {
+    case MURM_F32: return run<float>(g, count, ws, st);
+    case MURM_F16: return run<__half>(g, count, ws, st);
+    default: return run<__nv_bfloat16>(g, count, ws, st);
   }
 }
 

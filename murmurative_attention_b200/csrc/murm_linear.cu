@@ -7,6 +7,7 @@
 #include <cstdio>
 
 #include "murm_linear.cuh"
+#include "murm_sm100.cuh"
 
 namespace murm {
 namespace lin {
@@ -68,6 +69,8 @@ template <typename T, int V, bool SLOPE>
 __global__ void __launch_bounds__(kDzThreads, 3)
     k_dz(const T* dy, int64_t ldy, const Slope<T>* slope, int M, int N, int cols, int chunk, Operand dz, float* part) {
   __shared__ float s[kDzThreads * V];  // [row group][column]
+  sm100::pdl_wait();
+  sm100::pdl_trigger();
   const int tx = threadIdx.x & (cols - 1), ty = threadIdx.x / cols, rows = kDzThreads / cols;
   const int n = (blockIdx.x * cols + tx) * V;
   const int m1 = (int)min((int64_t)M, (int64_t)(blockIdx.y + 1) * chunk);
@@ -129,6 +132,8 @@ __global__ void __launch_bounds__(kDzThreads, 3)
 template <typename T>
 __global__ void __launch_bounds__(256) k_col_sum(const float* part, int chunks, int N, T* out) {
   __shared__ float s[8][33];
+  sm100::pdl_wait();
+  sm100::pdl_trigger();
   const int n = blockIdx.x * 32 + (threadIdx.x & 31), ty = threadIdx.x >> 5;
   float sum = 0.f;
   if (n < N)
@@ -157,13 +162,13 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
   const dim3 grid(blocks_x, chunks);
   const T* dy = static_cast<const T*>(a.grad_out);
   if (a.activation == MURM_ACT_NONE)
-    MURM_LAUNCH("linear_col_part", (k_dz<T, V, false>), grid, kDzThreads, 0, st, dy, a.go_stride,
+    MURM_LAUNCH_PDL("linear_col_part", (k_dz<T, V, false>), grid, kDzThreads, 0, st, dy, a.go_stride,
                 (const Slope<T>*)nullptr, M, N, cols, chunk, dz, part);
   else
-    MURM_LAUNCH("linear_dz", (k_dz<T, V, true>), grid, kDzThreads, 0, st, dy, a.go_stride,
+    MURM_LAUNCH_PDL("linear_dz", (k_dz<T, V, true>), grid, kDzThreads, 0, st, dy, a.go_stride,
                 static_cast<const Slope<T>*>(a.slope), M, N, cols, chunk, dz, part);
   if (part)
-    MURM_LAUNCH("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 256, 0, st, (const float*)part, chunks, N,
+    MURM_LAUNCH_PDL("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 256, 0, st, (const float*)part, chunks, N,
                 static_cast<T*>(a.grad_bias));
 }
 
@@ -292,7 +297,7 @@ FwdPlan plan_fwd(const murm_linear_args& a) {
   g.out = a.out; g.ldo = a.out_stride;
   g.slope = a.slope;
   g.act = a.activation;
-  p.gemm_at = p.l.take(gemm_workspace(g));
+  p.gemm_at = p.l.take(gemm_workspace(&g, 1));
   return p;
 }
 
@@ -302,7 +307,8 @@ struct BwdPlan {
   Source x, w, dy;  // dy: dz itself without an activation
   Operand dz;
   size_t part_at, gemm_at;
-  Gemm gx, gw;
+  Gemm g[2];  // dx, dW: those that are wanted
+  int count;
 };
 BwdPlan plan_bwd(const murm_linear_bwd_args& a) {
   BwdPlan p{};
@@ -328,24 +334,22 @@ BwdPlan plan_bwd(const murm_linear_bwd_args& a) {
   g.a = p.dz;
   g.N = a.in_features;
   g.b_mn = true;
-  size_t most = 0;
   if (a.grad_x) {
-    p.gx = g;
-    p.gx.b = p.w.op;
-    p.gx.M = (int)a.rows; p.gx.K = a.out_features;
-    p.gx.out = a.grad_x; p.gx.ldo = a.gx_stride;
-    most = gemm_workspace(p.gx);
+    Gemm& x = p.g[p.count++];
+    x = g;
+    x.b = p.w.op;
+    x.M = (int)a.rows; x.K = a.out_features;
+    x.out = a.grad_x; x.ldo = a.gx_stride;
   }
   if (a.grad_weight) {
-    p.gw = g;
-    p.gw.a_mn = true;
-    p.gw.b = p.x.op;
-    p.gw.M = a.out_features; p.gw.K = (int)a.rows;
-    p.gw.out = a.grad_weight; p.gw.ldo = a.gw_stride;
-    const size_t w = gemm_workspace(p.gw);
-    most = w > most ? w : most;
+    Gemm& w = p.g[p.count++];
+    w = g;
+    w.a_mn = true;
+    w.b = p.x.op;
+    w.M = a.out_features; w.K = (int)a.rows;
+    w.out = a.grad_weight; w.ldo = a.gw_stride;
   }
-  p.gemm_at = p.l.take(most);
+  p.gemm_at = p.l.take(p.count ? gemm_workspace(p.g, p.count) : 0);
   return p;
 }
 
@@ -355,7 +359,7 @@ murm_status run_fwd(const murm_linear_args& a, cudaStream_t st) {
   if (murm_status s = check_ws(a.workspace, a.workspace_bytes, p.l.bytes)) return s;
   if (murm_status s = fill(p.x, p.l, st)) return s;
   if (murm_status s = fill(p.w, p.l, st)) return s;
-  return gemm(p.g, p.l.ws + p.gemm_at, st);
+  return gemm(&p.g, 1, p.l.ws + p.gemm_at, st);
 }
 
 murm_status run_bwd(const murm_linear_bwd_args& a, cudaStream_t st) {
@@ -383,11 +387,7 @@ murm_status run_bwd(const murm_linear_bwd_args& a, cudaStream_t st) {
   if (murm_status s = fill(p.dy, p.l, st)) return s;
   if (murm_status s = fill(p.w, p.l, st)) return s;
   if (murm_status s = fill(p.x, p.l, st)) return s;
-  if (a.grad_x)
-    if (murm_status s = gemm(p.gx, p.l.ws + p.gemm_at, st)) return s;
-  if (a.grad_weight)
-    if (murm_status s = gemm(p.gw, p.l.ws + p.gemm_at, st)) return s;
-  return MURM_OK;
+  return p.count ? gemm(p.g, p.count, p.l.ws + p.gemm_at, st) : MURM_OK;
 }
 
 }  // namespace

@@ -28,8 +28,10 @@ struct Gemm {
   void* slope;   // [M][N] contiguous: act'(z) as Slope<T>, or NULL
   int act;       // murm_activation
 };
-size_t gemm_workspace(const Gemm& g);
-murm_status gemm(const Gemm& g, void* workspace, cudaStream_t st);
+// One product, or two that do not depend on each other (the backward's) in one launch where that is
+// the shorter way: their tiles fill the SMs together.
+size_t gemm_workspace(const Gemm* g, int count);
+murm_status gemm(const Gemm* g, int count, void* workspace, cudaStream_t st);
 
 // Type of the saved slopes: fp16 beside 16-bit tensors (slopes are of order one, so it holds them
 // eight times nearer than bf16 would), fp32 beside fp32.
