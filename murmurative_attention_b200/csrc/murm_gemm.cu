@@ -556,14 +556,22 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     k_split_sum(const float* part, int64_t split_stride, int ldp, const __grid_constant__ Args p) {
   pdl_wait();
+  pdl_trigger();
   const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
   const int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
   if (n >= p.N || m >= p.M) return;
   const float* src = part + m * ldp + n;
-  float4 s = *reinterpret_cast<const float4*>(src);
-  for (int i = 1; i < p.splits; ++i) {
-    const float4 v = *reinterpret_cast<const float4*>(src + i * split_stride);
-    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.splits; i += 4) {  // four splits' loads together, added in order
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = *reinterpret_cast<const float4*>(src + (int64_t)min(i + j, p.splits - 1) * split_stride);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j >= p.splits) break;
+      s.x += v[j].x; s.y += v[j].y; s.z += v[j].z; s.w += v[j].w;
+    }
   }
   float z[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -580,25 +588,41 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // packing
 // ---------------------------------------------------------------------------
-// Eight columns per thread; dst rows of `pitch` elements, the columns past `cols` zero.
+struct PackOne {
+  const void* src;
+  uint16_t* dst;  // rows of `pitch` elements, the columns past `cols` zero
+  int64_t ld, rows, plane;
+  int cols, pitch, vec, first;  // vec: 16-byte loads; first: the matrix's first block
+};
+struct PackArgs {
+  PackOne m[kMaxPack];
+  int count;
+};
+// Eight columns per thread and step; a run of blocks per matrix.
 template <typename T>
-__global__ void __launch_bounds__(256) k_pack(const T* src, int64_t ld, int64_t rows, int cols, uint16_t* dst, int pitch,
-                                              int64_t plane, int vec) {
-  pdl_wait();
-  const int64_t groups = (int64_t)rows * (pitch / 8);
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < groups; i += gridDim.x * 256ll) {
-    const int64_t r = i / (pitch / 8);
-    const int c = (int)(i - r * (pitch / 8)) * 8;
-    const T* s = src + r * ld + c;
+__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackArgs args) {
+  sm100::pdl_wait();
+  sm100::pdl_trigger();
+  int which = 0;
+  while (which + 1 < args.count && (int)blockIdx.x >= args.m[which + 1].first) ++which;
+  const PackOne& p = args.m[which];
+  const int blocks = (which + 1 < args.count ? args.m[which + 1].first : (int)gridDim.x) - p.first;
+  const int per_row = p.pitch / 8;
+  const int64_t groups = p.rows * per_row;
+  for (int64_t i = ((int)blockIdx.x - p.first) * 256ll + threadIdx.x; i < groups; i += blocks * 256ll) {
+    const int64_t r = i / per_row;
+    const int c = (int)(i - r * per_row) * 8;
+    const T* s = static_cast<const T*>(p.src) + r * p.ld + c;
+    uint16_t* dst = p.dst + r * p.pitch + c;
     alignas(16) uint16_t o[3][8];
     if constexpr (sizeof(T) == 4) {
       float v[8];
-      if (vec) {
+      if (p.vec) {
         *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(s);
         *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(s + 4);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? s[e] : 0.f;
+        for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? s[e] : 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -608,11 +632,11 @@ __global__ void __launch_bounds__(256) k_pack(const T* src, int64_t ld, int64_t 
       }
 #pragma unroll
       for (int q = 0; q < 3; ++q)
-        *reinterpret_cast<uint4*>(dst + q * plane + r * pitch + c) = *reinterpret_cast<const uint4*>(o[q]);
+        *reinterpret_cast<uint4*>(dst + q * p.plane) = *reinterpret_cast<const uint4*>(o[q]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[0][e] = c + e < cols ? *reinterpret_cast<const uint16_t*>(s + e) : 0;
-      *reinterpret_cast<uint4*>(dst + r * pitch + c) = *reinterpret_cast<const uint4*>(o[0]);
+      for (int e = 0; e < 8; ++e) o[0][e] = c + e < p.cols ? *reinterpret_cast<const uint16_t*>(s + e) : 0;
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o[0]);
     }
   }
 }
@@ -913,19 +937,19 @@ Operand packed_at(int dtype, const Matrix& m, void* dst) {
   return Operand{dst, pitch_of(m.cols), m.rows * pitch_of(m.cols), dtype == MURM_F32 ? 3 : 1};
 }
 
-murm_status pack(int dtype, const Matrix& m, void* dst, cudaStream_t st) {
-  const int pitch = (int)pitch_of(m.cols);
-  const int64_t plane = m.rows * pitch;
-  int64_t blocks = (m.rows * (pitch / 8) + 255) / 256;
-  if (blocks > kSms * 16) blocks = kSms * 16;
-  if (dtype == MURM_F32) {
-    const int vec = m.cols % 8 == 0 && tma_rows(m.p, m.ld, 4);
-    launch("linear_pack", k_pack<float>, dim3((unsigned)blocks), 256, 0, st, static_cast<const float*>(m.p), m.ld, m.rows,
-           m.cols, static_cast<uint16_t*>(dst), pitch, plane, vec);
-  } else {
-    launch("linear_pack", k_pack<__half>, dim3((unsigned)blocks), 256, 0, st, static_cast<const __half*>(m.p), m.ld,
-           m.rows, m.cols, static_cast<uint16_t*>(dst), pitch, plane, 0);
+murm_status pack(int dtype, const Matrix* m, void* const* dst, int count, cudaStream_t st) {
+  PackArgs a{};
+  a.count = count;
+  int64_t blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    const int pitch = (int)pitch_of(m[i].cols);
+    a.m[i] = PackOne{m[i].p, static_cast<uint16_t*>(dst[i]), m[i].ld, m[i].rows, m[i].rows * pitch, m[i].cols, pitch,
+                     dtype == MURM_F32 && m[i].cols % 8 == 0 && tma_rows(m[i].p, m[i].ld, 4), (int)blocks};
+    const int64_t need = (m[i].rows * (pitch / 8) + 255) / 256;
+    blocks += need < kSms * 16 ? need : kSms * 16;
   }
+  if (dtype == MURM_F32) launch("linear_pack", k_pack<float>, dim3((unsigned)blocks), 256, 0, st, a);
+  else launch("linear_pack", k_pack<__half>, dim3((unsigned)blocks), 256, 0, st, a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MURM_OK : report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -5,6 +5,7 @@
 // pass over both, then dx = dz W and dW = dz^T x. Without an activation dz is dy itself and the pass only sums it.
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 
 #include "murm_linear.cuh"
 #include "murm_sm100.cuh"
@@ -271,8 +272,16 @@ struct Layout {
     return s;
   }
 };
-murm_status fill(const Source& s, const Layout& l, cudaStream_t st) {
-  return s.packed ? pack(l.dtype, s.m, l.ws + s.at, st) : MURM_OK;
+murm_status fill(std::initializer_list<const Source*> all, const Layout& l, cudaStream_t st) {
+  Matrix m[kMaxPack];
+  void* dst[kMaxPack];
+  int count = 0;
+  for (const Source* s : all) {
+    if (!s->packed) continue;
+    m[count] = s->m;
+    dst[count++] = l.ws + s->at;
+  }
+  return count ? pack(l.dtype, m, dst, count, st) : MURM_OK;
 }
 
 struct FwdPlan {
@@ -357,8 +366,7 @@ murm_status run_fwd(const murm_linear_args& a, cudaStream_t st) {
   if (few_rows(a)) return few_rows_forward(a, st);
   const FwdPlan p = plan_fwd(a);
   if (murm_status s = check_ws(a.workspace, a.workspace_bytes, p.l.bytes)) return s;
-  if (murm_status s = fill(p.x, p.l, st)) return s;
-  if (murm_status s = fill(p.w, p.l, st)) return s;
+  if (murm_status s = fill({&p.x, &p.w}, p.l, st)) return s;
   return gemm(&p.g, 1, p.l.ws + p.gemm_at, st);
 }
 
@@ -384,9 +392,7 @@ murm_status run_bwd(const murm_linear_bwd_args& a, cudaStream_t st) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return bad(MURM_ERR_CUDA, "linear backward launch: %s", cudaGetErrorString(e));
   }
-  if (murm_status s = fill(p.dy, p.l, st)) return s;
-  if (murm_status s = fill(p.w, p.l, st)) return s;
-  if (murm_status s = fill(p.x, p.l, st)) return s;
+  if (murm_status s = fill({&p.dy, &p.w, &p.x}, p.l, st)) return s;
   return p.count ? gemm(p.g, p.count, p.l.ws + p.gemm_at, st) : MURM_OK;
 }
 

@@ -54,7 +54,9 @@ struct Matrix {
 bool needs_pack(int dtype, const Matrix& m);
 size_t pack_bytes(int dtype, const Matrix& m);
 Operand packed_at(int dtype, const Matrix& m, void* dst);  // the operand pack() writes at dst
-murm_status pack(int dtype, const Matrix& m, void* dst, cudaStream_t st);
+constexpr int kMaxPack = 3;
+// Up to kMaxPack matrices in one launch.
+murm_status pack(int dtype, const Matrix* m, void* const* dst, int count, cudaStream_t st);
 
 // ---------------------------------------------------------------------------
 // activations, in fp32
