@@ -570,6 +570,36 @@ Tensor rotary(const Tensor& x, const Tensor& positions, double base, optional<in
                       inverse);
 }
 
+// ---------------------------------------------------------------------------
+// the passes without autograd, for the registered operators (torch_ops.py)
+// ---------------------------------------------------------------------------
+Tensor or_empty(const Tensor& t, const Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
+
+std::tuple<Tensor, Tensor> linear_fwd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
+                                      const std::string& activation, const optional<Tensor>& residual) {
+  auto [out, slope] = linear_forward(x, weight, value(bias), value(residual), activation_code(activation), true);
+  return {out, or_empty(slope, x)};
+}
+std::tuple<Tensor, Tensor, Tensor> linear_bwd(const Tensor& go, const Tensor& x, const Tensor& weight,
+                                              const Tensor& slope, const std::string& activation) {
+  return linear_backward(go, x, weight, slope.numel() ? slope : Tensor(), activation_code(activation), true, true, true);
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_bwd(const Tensor& gq, const Tensor& gk, const Tensor& q,
+                                                  const optional<Tensor>& k_, const Tensor& positions,
+                                                  const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
+                                                  double eps, double base, optional<int64_t> rotary_dim,
+                                                  bool interleaved, const optional<std::vector<int64_t>>& sections,
+                                                  const std::string& spectrum, const optional<Tensor>& freqs) {
+  const Tensor k = value(k_);
+  const Tensor x[2] = {q, k};
+  const Tensor w[2] = {gain(q_weight, q, "q_weight"), k.defined() ? gain(k_weight, k, "k_weight") : Tensor()};
+  const Tensor go[2] = {gq, gk};
+  const bool need[2] = {true, k.defined()};
+  const auto res = norm_rope_backward(
+      x, w, go, need, make_rotation(q, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, eps));
+  return {res[0], or_empty(res[1], q), or_empty(res[2], q), or_empty(res[3], q)};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_murm_torch, m) {
@@ -578,4 +608,7 @@ PYBIND11_MODULE(_murm_torch, m) {
   m.def("fused_linear", &fused_linear);
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("rotary", &rotary);
+  m.def("linear_fwd", &linear_fwd);
+  m.def("linear_bwd", &linear_bwd);
+  m.def("qk_bwd", &qk_bwd);
 }

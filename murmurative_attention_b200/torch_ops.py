@@ -18,7 +18,9 @@ It also defines the north-star operation of this library as an operator with aut
         -> (Tensor out, Tensor indices, Tensor weights)
 
 built from ``slot_murmurate_fwd`` (which also returns the block the backward reads) and
-``slot_murmurate_bwd``, both on the fused tensor-core C ABI. Every operator has a fake
+``slot_murmurate_bwd``, both on the fused tensor-core C ABI, and the block's operators around it
+with their gradients (``fused_linear_fwd`` / ``_bwd``, ``qk_norm_rope`` / ``_bwd``, ``rotary``), which
+``fused_linear``, ``qk_norm_rope`` and ``rotary`` call while torch.compile traces them. Every operator has a fake
 (meta) implementation, so FakeTensor tracing and ``torch.compile(fullgraph=True)`` see
 through them; the sizes the fakes need come from the library's host-only size functions.
 There is no CPU kernel: like the reference's ops, these run on CUDA tensors only.
@@ -30,7 +32,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from . import _lib, functional, ops
+from . import _lib, _native, functional, ops
 
 NS = "murmurative_attention"
 
@@ -65,8 +67,23 @@ NORTH_STAR_SCHEMAS = {
                       "(Tensor, Tensor, Tensor)",
 }
 
+_ROTATION = ("float eps, float base, int? rotary_dim, bool interleaved, int[]? sections, str spectrum, "
+             "Tensor? freqs")
+BLOCK_SCHEMAS = {
+    "fused_linear_fwd": "fused_linear_fwd(Tensor x, Tensor weight, Tensor? bias, str activation, Tensor? residual) "
+                        "-> (Tensor, Tensor)",
+    "fused_linear_bwd": "fused_linear_bwd(Tensor grad_out, Tensor x, Tensor weight, Tensor slope, str activation) "
+                        "-> (Tensor, Tensor, Tensor)",
+    "qk_norm_rope": f"qk_norm_rope(Tensor q, Tensor? k, Tensor positions, Tensor? q_weight, Tensor? k_weight, "
+                    f"{_ROTATION}) -> (Tensor, Tensor)",
+    "qk_norm_rope_bwd": f"qk_norm_rope_bwd(Tensor grad_q, Tensor grad_k, Tensor q, Tensor? k, Tensor positions, "
+                        f"Tensor? q_weight, Tensor? k_weight, {_ROTATION}) -> (Tensor, Tensor, Tensor, Tensor)",
+    "rotary": "rotary(Tensor x, Tensor positions, float base, int? rotary_dim, bool interleaved, int[]? sections, "
+              "str spectrum, Tensor? freqs, bool inverse) -> Tensor",
+}
+
 _LIB = torch.library.Library(NS, "DEF")
-for _schema in list(REFERENCE_SCHEMAS.values()) + list(NORTH_STAR_SCHEMAS.values()):
+for _schema in list(REFERENCE_SCHEMAS.values()) + list(NORTH_STAR_SCHEMAS.values()) + list(BLOCK_SCHEMAS.values()):
     _LIB.define(_schema)
 
 
@@ -247,3 +264,130 @@ def slot_murmurate(q: Tensor, slots_k: Tensor, slots_v: Tensor, rounds: int = 3,
     torch.compile)."""
     return torch.ops.murmurative_attention.slot_murmurate(q, slots_k, slots_v, rounds, top_k, causal, alpha, gamma,
                                                           scale)
+
+
+# ---------------------------------------------------------------------------
+# The block's operators (compiled binding over the C ABI)
+# ---------------------------------------------------------------------------
+@torch.library.impl(_q("fused_linear_fwd"), "CUDA", lib=_LIB)
+def _linear_fwd_cuda(x, weight, bias, activation, residual):
+    return _native.binding().linear_fwd(x, weight, bias, activation, residual)
+
+
+@torch.library.register_fake(_q("fused_linear_fwd"), lib=_LIB)
+def _linear_fwd_fake(x, weight, bias, activation, residual):
+    out = x.new_empty(x.shape[0], weight.shape[0])
+    if activation == "none":
+        return out, x.new_empty(0)
+    return out, torch.empty_like(out, dtype=torch.float32 if x.dtype == torch.float32 else torch.float16)
+
+
+@torch.library.impl(_q("fused_linear_bwd"), "CUDA", lib=_LIB)
+def _linear_bwd_cuda(grad_out, x, weight, slope, activation):
+    return _native.binding().linear_bwd(grad_out, x, weight, slope, activation)
+
+
+@torch.library.register_fake(_q("fused_linear_bwd"), lib=_LIB)
+def _linear_bwd_fake(grad_out, x, weight, slope, activation):
+    return x.new_empty(x.shape), x.new_empty(weight.shape), x.new_empty(weight.shape[0])
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, activation, residual = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.activation, ctx.has = activation, (bias is not None, residual is not None)
+    ctx.mark_non_differentiable(output[1])
+
+
+def _linear_backward(ctx, grad_out, grad_slope):
+    x, weight, slope = ctx.saved_tensors
+    gx, gw, gb = torch.ops.murmurative_attention.fused_linear_bwd(grad_out, x, weight, slope, ctx.activation)
+    return gx, gw, gb if ctx.has[0] else None, None, grad_out if ctx.has[1] else None
+
+
+torch.library.register_autograd(_q("fused_linear_fwd"), _linear_backward, setup_context=_linear_setup, lib=_LIB)
+
+
+def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: str,
+                 residual: Optional[Tensor]) -> Tensor:
+    """The registered form of ``fused_linear`` (same operation; traceable by torch.compile)."""
+    shape = x.shape[:-1] + (weight.shape[0],)
+    x2 = x.reshape(-1, x.shape[-1])
+    r2 = residual.expand(shape).reshape(-1, shape[-1]) if residual is not None else None
+    out, _ = torch.ops.murmurative_attention.fused_linear_fwd(x2, weight, bias, activation, r2)
+    return out.view(shape)
+
+
+def _unit_layout(t: Tensor) -> Tensor:
+    """An empty tensor as the rotation's results are laid out: like the rows when their inner stride is 1."""
+    return torch.empty_like(t if t.stride(3) == 1 else t.contiguous())
+
+
+@torch.library.impl(_q("qk_norm_rope"), "CUDA", lib=_LIB)
+def _qk_cuda(q, k, positions, q_weight, k_weight, *rotation):
+    with torch.no_grad():
+        oq, ok = _native.binding().qk_norm_rope(q, k, positions, q_weight, k_weight, *rotation)
+    return oq, ok if ok is not None else q.new_empty(0)
+
+
+@torch.library.register_fake(_q("qk_norm_rope"), lib=_LIB)
+def _qk_fake(q, k, positions, q_weight, k_weight, *rotation):
+    return _unit_layout(q), _unit_layout(k) if k is not None else q.new_empty(0)
+
+
+@torch.library.impl(_q("qk_norm_rope_bwd"), "CUDA", lib=_LIB)
+def _qk_bwd_cuda(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation):
+    return _native.binding().qk_bwd(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation)
+
+
+@torch.library.register_fake(_q("qk_norm_rope_bwd"), lib=_LIB)
+def _qk_bwd_fake(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation):
+    none = q.new_empty(0)
+    return (_unit_layout(q), _unit_layout(k) if k is not None else none,
+            torch.empty_like(q_weight) if q_weight is not None else none,
+            torch.empty_like(k_weight) if k_weight is not None else none)
+
+
+def _qk_setup(ctx, inputs, output):
+    q, k, positions, q_weight, k_weight, eps, base, rotary_dim, interleaved, sections, spectrum, freqs = inputs
+    ctx.save_for_backward(q, k, positions, q_weight, k_weight, freqs)
+    ctx.rotation = (eps, base, rotary_dim, interleaved, sections, spectrum)
+
+
+def _qk_backward(ctx, grad_q, grad_k):
+    q, k, positions, q_weight, k_weight, freqs = ctx.saved_tensors
+    gq, gk, gqw, gkw = torch.ops.murmurative_attention.qk_norm_rope_bwd(
+        grad_q if grad_q is not None else torch.zeros_like(q),
+        grad_k if grad_k is not None else torch.zeros_like(k if k is not None else q), q, k, positions, q_weight,
+        k_weight, *ctx.rotation, freqs)
+    return (gq, gk if k is not None else None, None, gqw if q_weight is not None else None,
+            gkw if k_weight is not None else None) + (None,) * 7
+
+
+torch.library.register_autograd(_q("qk_norm_rope"), _qk_backward, setup_context=_qk_setup, lib=_LIB)
+
+
+@torch.library.impl(_q("rotary"), "CUDA", lib=_LIB)
+def _rotary_cuda(x, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, inverse):
+    with torch.no_grad():
+        return _native.binding().rotary(x, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, inverse)
+
+
+@torch.library.register_fake(_q("rotary"), lib=_LIB)
+def _rotary_fake(x, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, inverse):
+    return _unit_layout(x)
+
+
+def _rotary_setup(ctx, inputs, output):
+    x, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, inverse = inputs
+    ctx.save_for_backward(positions, freqs)
+    ctx.rotation = (base, rotary_dim, interleaved, sections, spectrum)
+    ctx.inverse = inverse
+
+
+def _rotary_backward(ctx, grad):
+    positions, freqs = ctx.saved_tensors
+    return (torch.ops.murmurative_attention.rotary(grad, positions, *ctx.rotation, freqs, not ctx.inverse),) + (None,) * 8
+
+
+torch.library.register_autograd(_q("rotary"), _rotary_backward, setup_context=_rotary_setup, lib=_LIB)
