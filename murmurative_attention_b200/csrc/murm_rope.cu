@@ -802,7 +802,7 @@ murm_status check_rows(const murm_norm_rope_args& a, const murm_head_rows& r, co
                          (backward ? reinterpret_cast<uintptr_t>(r.grad) : 0);
   if (bits % es) return bad(MURM_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its element", name);
   for (int i = 0; i < 3; ++i)
-    if (r.out_stride[i] == 0 && (i == 0 ? a.batch : i == 1 ? r.heads : a.tokens) > 1)
+    if (!empty && r.out_stride[i] == 0 && (i == 0 ? a.batch : i == 1 ? r.heads : a.tokens) > 1)
       return bad(MURM_ERR_INVALID_ARGUMENT, "%s: out stride[%d] is zero", name, i);
   if ((r.weight || r.grad_weight) && r.weight_dtype != MURM_F32 && r.weight_dtype != a.dtype)
     return bad(MURM_ERR_DTYPE, "%s weight must be fp32 or of the rows' dtype, got code %d", name, r.weight_dtype);
