@@ -6,8 +6,10 @@
 //
 // k_gemm_tc: a pair of CTAs (cta_group::2) per 256 x BN tile, each holding 128 rows of A, half the
 // rows of B and a 128 x BN fp32 accumulator in TMEM (two accumulators: a tile's epilogue runs under
-// the next tile's products). Persistent over the tiles. Warp 0 loads the operands by TMA into a
-// ring of 64-deep stages, warp 1 of the first CTA issues the MMAs of both, warps 4-19 run the
+// the next tile's products). Persistent over the tiles. Warps 0, 2 and 3 load the operands by TMA into
+// a ring of 64-deep stages, a stage each in turn (one thread needs some 490 clocks to wait for a stage
+// and issue its copies, as long as the MMAs take), warp 1 of the first CTA issues the MMAs of both
+// CTAs, warps 4-19 run the
 // epilogue, each on 32 rows and a quarter of the columns: TMEM -> registers -> bias, activation,
 // residual -> 64-byte swizzled rows in shared memory -> TMA store (or plain stores where the
 // result's rows are not 16-byte aligned).
@@ -36,6 +38,7 @@ constexpr int kSms = 148;
 constexpr int kPairs = kSms / 2;     // CTA pairs resident at once
 constexpr int kBK = 64;              // depth of a stage: one 128-byte swizzled row
 constexpr uint32_t kABytes = 128 * kBK * 2;
+constexpr int kLoaders = 3;
 constexpr int kEpiWarps = 16;        // 4 row groups (TMEM lanes) x 4 column groups
 constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr uint32_t kBuf = 32 * 64;   // one epilogue warp's 32 rows of 64 bytes
@@ -100,8 +103,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// Both CTAs have come here. Relaxed: what has to be seen across (barrier initialisation) has a fence
+// of its own; a releasing arrival waits some 1000 clocks for the thread's global stores.
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The address of the first CTA's copy of a shared-memory object.
 __device__ __forceinline__ uint32_t map_to_first(const void* p) {
@@ -109,8 +114,13 @@ __device__ __forceinline__ uint32_t map_to_first(const void* p) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
   return r;
 }
+// Says that this warp's reads of TMEM are done (ordered by the tcgen05 fence before it; relaxed for
+// the same reason as above).
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // Load into this CTA's shared memory that counts on a barrier of the pair's first CTA.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
@@ -359,32 +369,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_barrier_init();
   }
   if (warp == 2) tmem_alloc_pair(&bars->tmem, L::kTmemCols);
+  if (warp == 3 && lane < (TWO ? 2 : 1)) {
+    prefetch_map(&l.q[lane].a);
+    prefetch_map(&l.q[lane].b);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are up before any remote arrival
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
-  pdl_wait();
   pdl_trigger();
 
-  if (warp == 0 && lane == 0) {
+  if (warp < 4 && warp != 1 && lane == 0) {
     // ------------------------------------------------------------ operand loads
-    uint32_t s = 0, ph = 0;  // stage and its round's parity
-    int issued = 0;
+    const int mine = warp ? warp - 1 : 0;  // this loader's stages: mine, mine + kLoaders, ...
+    const uint32_t full0 = map_to_first(&bars->full[0]);
+    int base = 0;  // stages of the items before
     bool ok = true;
+    Item t = item_at<BN, TWO>(l, first);  // the parameters come from a cold constant cache: before the wait
+    pdl_wait();
     for (int at = first; ok && at < l.positions; at += step) {
-      const Item t = item_at<BN, TWO>(l, at);
+      if (at != first) t = item_at<BN, TWO>(l, at);
       if (t.which < 0) continue;
       const Problem& pr = l.q[TWO ? t.which : 0];
       const CUtensorMap *map_a = &pr.a, *map_b = &pr.b;
       const int a_mn = pr.p.a_mn, b_mn = pr.p.b_mn, fp32 = pr.p.fp32, kblocks = pr.p.kblocks;
       const int ma = t.m0 + (int)rank * 128, nb = t.n0 + (int)rank * (BN / 2);
-      int pair = fp32 ? t.i0 / kblocks : 0;
-      int kb = t.i0 - pair * kblocks;
-      for (int i = t.i0; i < t.i1; ++i) {
+      const int skip = (mine + kLoaders - base % kLoaders) % kLoaders;
+      int s = (base + skip) % L::kStages;
+      uint32_t ph = ((base + skip) / L::kStages) & 1;  // the parity of the stage's round
+      int pair = fp32 ? (t.i0 + skip) / kblocks : 0;
+      int kb = t.i0 + skip - pair * kblocks;
+      for (int i = t.i0 + skip; i < t.i1; i += kLoaders) {
         if (!(ok = wait(&bars->empty[s], ph ^ 1))) break;
         if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
-        const uint32_t bar = map_to_first(&bars->full[s]);
+        const uint32_t bar = full0 + s * 8;
         const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
         const int k = kb * kBK;
         const int pa = fp32 ? plane_a(pair) : 0, pb = fp32 ? plane_b(pair) : 0;
@@ -400,13 +419,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         } else {
           tma_load_pair(sb, map_b, k, nb, pb, bar);
         }
-        ++issued;
-        if (++kb == kblocks) { kb = 0; ++pair; }
-        if (++s == L::kStages) { s = 0; ph ^= 1; }
+        kb += kLoaders;
+        while (fp32 && kb >= kblocks) { kb -= kblocks; ++pair; }
+        s += kLoaders;
+        if (s >= L::kStages) { s -= L::kStages; ph ^= 1; }
       }
+      base += t.i1 - t.i0;
     }
     // the last stages' loads and releases must have arrived before the CTAs may exit
-    for (int j = max(0, issued - L::kStages); j < issued; ++j) {
+    for (int j = max(0, base - L::kStages); mine == 0 && j < base; ++j) {
       const int st = j % L::kStages, par = (j / L::kStages) & 1;
       if (rank == 0 && !wait(&bars->full[st], par)) break;
       if (ok) ok = wait(&bars->empty[st], par);
@@ -454,6 +475,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int w = warp & 3, quarter = (warp - 4) >> 2;  // TMEM lanes 32w.., columns quarter * BN/4..
     const uint32_t sbuf = sbase + L::OFF_OUT + (warp - 4) * kBuf;
     uint8_t* pbuf = smem + L::OFF_OUT + (warp - 4) * kBuf;
+    pdl_wait();
     int t = 0;
     bool ok = true;
     // sends the buffer's rows out, once every lane has written its own
