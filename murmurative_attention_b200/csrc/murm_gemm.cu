@@ -46,7 +46,7 @@ constexpr uint32_t kBuf = 32 * 64;   // one epilogue warp's 32 rows of 64 bytes
 template <int BN> struct Tile {
   static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
   static constexpr uint32_t kStage = kABytes + kBBytes;
-  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kStages = BN == 256 ? 6 : 8;  // of 256: 6 and 5 alike, 4 3 % slower
   static constexpr uint32_t OFF_OUT = kStages * kStage;  // one buffer per epilogue warp
   static constexpr uint32_t OFF_BAR = OFF_OUT + kEpiWarps * kBuf;
   static constexpr uint32_t kSmem = OFF_BAR + 256 + 1024;
@@ -685,15 +685,15 @@ Config config(const Gemm& g, int bn, int splits) {
 }
 
 // Tile width and K splits by estimated time, in microseconds measured on B200:
-// - a 64-deep stage takes 0.35 of a 256-wide tile (its 64 KB per CTA pair are about what L2 delivers
-//   to two SMs in that time, which is also the MMAs' own) and 0.31 of a 128-wide one, bound by the
-//   rows of A it loads all the same; 15 % more where A is read MN-major. So 128 pays only where it
-//   leaves fewer rounds: 512 x 1024 x 1024: 9.5 us at 128, 10.2 at 256; 8192 x 1024 x 1024: 27.5 and 18.1.
+// - with all pairs busy a 64-deep stage takes 0.35 of a 256-wide tile and 0.31 of a 128-wide one (its
+//   MMAs take half as long, but the wait for a stage, its MMAs' issue and its release do not). So 128
+//   pays only where it leaves fewer rounds: 512 x 1024 x 1024: 8.9 us at 128, 9.8 at 256;
+//   8192 x 1024 x 1024: 25.9 and 16.7.
 // - a split costs a second launch, and its fp32 sums about 4.8 MB per us:
-//   1024 x 1024 x 8192 (dW): 50 us in one part, 24 in four, 28 in eight.
+//   1024 x 1024 x 8192 (dW): 24 us in three parts, 21 in four, 24 in eight.
 // - a launch of its own costs about 5 (prologue, first loads, last epilogue).
 constexpr double kLaunchUs = 5.0;
-double stage_us(const Gemm& g, int bn) { return (bn == 256 ? 0.35 : 0.31) * (g.a_mn ? 1.15 : 1.0); }
+double stage_us(int bn) { return bn == 256 ? 0.35 : 0.31; }
 double split_us(const Config& c) {
   return c.splits == 1 ? 0.0 : 4.0 + (double)c.tiles_m * c.tiles_n * 256 * c.bn * 4 * c.splits / 4.8e6;
 }
@@ -707,7 +707,7 @@ double choose_one(const Gemm& g, Config* best) {
       const Config c = config(g, bn, splits);
       if (!split_fits(c, splits)) break;
       const int64_t rounds = ((int64_t)c.tiles_m * c.tiles_n * c.splits + kPairs - 1) / kPairs;
-      const double t = rounds * c.iters * stage_us(g, bn) + split_us(c);
+      const double t = rounds * c.iters * stage_us(bn) + split_us(c);
       if (best_t == 0 || t < best_t) {
         best_t = t;
         *best = c;
@@ -721,9 +721,10 @@ struct Plan {
   bool together;
 };
 // Two products together: no shorter than their work over all pairs, than the longest item, or than
-// what the last item of a pair leaves idle; side by side they also run a tenth slower than alone (two
-// sets of operands in L2, and no SM left idle whose power the others could use). It pays for short
-// products: both gradients of 8192 x 1024 x 1024 41.6 us, apart 45.6; of 32768 x 1024 x 4096 428 and 407.
+// what the last item of a pair leaves idle (about a quarter of the shorter ones); side by side they
+// also run a tenth slower than alone (two sets of operands in L2, and no SM left idle whose power the
+// others could use). Both gradients of 2048 x 1024 x 1024: 15.3 us, apart 23.9; of 8192 x 1024 x 1024
+// 33.7 and 39.3, of 4096 x 1024 x 4096 48.0 and 52.5, of 32768 x 1024 x 4096 406 and 378.
 constexpr double kTogether = 1.1;
 Plan choose(const Gemm* g, int count) {
   Plan p{};
@@ -742,7 +743,7 @@ Plan choose(const Gemm* g, int count) {
         Option& o = opt[i][n[i]];
         o.c = config(g[i], bn, splits);
         if (!split_fits(o.c, splits)) break;
-        o.item = o.c.iters * stage_us(g[i], bn);
+        o.item = o.c.iters * stage_us(bn);
         o.work = o.item * o.c.tiles_m * o.c.tiles_n * o.c.splits;
         o.extra = split_us(o.c);
         ++n[i];
@@ -750,7 +751,7 @@ Plan choose(const Gemm* g, int count) {
     for (int a = 0; a < n[0]; ++a)
       for (int b = 0; b < n[1]; ++b) {
         const Option &x = opt[0][a], &y = opt[1][b];
-        const double work = kTogether * (x.work + y.work) / kPairs + (x.item < y.item ? x.item : y.item) / 2;
+        const double work = kTogether * (x.work + y.work) / kPairs + (x.item < y.item ? x.item : y.item) / 4;
         const double longest = x.item > y.item ? x.item : y.item;
         const double t = kLaunchUs + x.extra + y.extra + (work > longest ? work : longest);
         if (t < apart) {
