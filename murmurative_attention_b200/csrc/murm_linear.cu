@@ -58,7 +58,7 @@ __device__ __forceinline__ void store_operand(const Operand& o, int64_t at, cons
 
 // Block (x, y): `cols` threads side by side (a power of two, as many as a row has groups of V
 // columns, up to the block), the others on further rows; a chunk of rows. db sums dz unrounded, in
-// fp32: a thread's rows in order, then the block's row groups in order, then (k_col_sum) the chunks.
+// fp32: a thread's rows in order, then the block's row groups in order, then (k_col_sum, if there are several) the chunks.
 //
 // Bound by memory: dy and the slopes read once, dz written once; 32768 x 4096 bf16 takes 129 us
 // (6.3 TB/s). A row's columns go to neighbouring threads and a thread issues kDzDepth rows' loads
@@ -68,7 +68,8 @@ constexpr int kDzDepth = 4;
 
 template <typename T, int V, bool SLOPE>
 __global__ void __launch_bounds__(kDzThreads, 3)
-    k_dz(const T* dy, int64_t ldy, const Slope<T>* slope, int M, int N, int cols, int chunk, Operand dz, float* part) {
+    k_dz(const T* dy, int64_t ldy, const Slope<T>* slope, int M, int N, int cols, int chunk, Operand dz, float* part,
+         T* db) {
   __shared__ float s[kDzThreads * V];  // [row group][column]
   sm100::pdl_wait();
   sm100::pdl_trigger();
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kDzThreads, 3)
       ps += (int64_t)rows * N;
     }
   }
-  if (!part) return;
+  if (!part && !db) return;
 #pragma unroll
   for (int e = 0; e < V; ++e) s[(ty * cols + tx) * V + e] = acc[e];
   __syncthreads();
@@ -126,7 +127,8 @@ __global__ void __launch_bounds__(kDzThreads, 3)
     if (col >= N) continue;
     float sum = 0.f;
     for (int r = 0; r < rows; ++r) sum += s[r * cols * V + c];
-    part[(int64_t)blockIdx.y * N + col] = sum;
+    if (db) Elem<T>::store(db + col, sum);  // the only chunk
+    else part[(int64_t)blockIdx.y * N + col] = sum;
   }
 }
 
@@ -158,16 +160,20 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
   int most = (148 * 6 + blocks_x - 1) / blocks_x;
   if (most > kDzChunks) most = kDzChunks;
   if (most > (M + 31) / 32) most = (M + 31) / 32;
+  // few rows per thread in all: one chunk, whose block writes db itself (a launch less)
+  if (M <= 16 * (kDzThreads / cols)) most = 1;
   const int chunk = (M + most - 1) / most;
   const int chunks = (M + chunk - 1) / chunk;
   const dim3 grid(blocks_x, chunks);
   const T* dy = static_cast<const T*>(a.grad_out);
+  T* db = part && chunks == 1 ? static_cast<T*>(a.grad_bias) : nullptr;
+  if (db) part = nullptr;
   if (a.activation == MURM_ACT_NONE)
     MURM_LAUNCH_PDL("linear_col_part", (k_dz<T, V, false>), grid, kDzThreads, 0, st, dy, a.go_stride,
-                (const Slope<T>*)nullptr, M, N, cols, chunk, dz, part);
+                (const Slope<T>*)nullptr, M, N, cols, chunk, dz, part, db);
   else
     MURM_LAUNCH_PDL("linear_dz", (k_dz<T, V, true>), grid, kDzThreads, 0, st, dy, a.go_stride,
-                static_cast<const Slope<T>*>(a.slope), M, N, cols, chunk, dz, part);
+                static_cast<const Slope<T>*>(a.slope), M, N, cols, chunk, dz, part, db);
   if (part)
     MURM_LAUNCH_PDL("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 256, 0, st, (const float*)part, chunks, N,
                 static_cast<T*>(a.grad_bias));
