@@ -15,8 +15,8 @@
 // once for all of them. The norm's kernels walk over their items with a ring of asynchronous copies
 // in shared memory ahead of them; the rotation, with a third of the arithmetic, takes an item per
 // group and several rows at once.
-// Measured: norm and rotation of q and k, 8 x 8192 tokens, 16 + 4 heads of 128, bf16: 123 us
-// (671 MB, 5.5 TB/s), backward 199 us (1.0 GB, 5.1 TB/s); rotation of 2 x 23400 x 24 rows of 128:
+// Measured: norm and rotation of q and k, 8 x 8192 tokens, 16 + 4 heads of 128, bf16: 121 us
+// (671 MB, 5.5 TB/s), backward 198 us (1.0 GB, 5.1 TB/s); rotation of 2 x 23400 x 24 rows of 128:
 // 91 us (575 MB, 6.3 TB/s).
 #include <cmath>
 #include <cstdarg>
@@ -33,16 +33,20 @@ constexpr int kMaxPairs = 128;
 constexpr int kMaxD = 256;
 constexpr int kSms = 148;
 // Launch shapes, by measurement (q and k of 8 x 8192 tokens, 16 + 4 heads of 128, bf16):
-// forward: 8 pairs per lane, 2 rows side by side, rings of 6, 2 blocks per SM: 123 us; 1 row 129,
-//   4 rows 137, 1 block 164, 4 pairs per lane 167 (more shuffles and addresses per byte);
-// backward: 8 pairs, 1 row, rings of 4, 2 blocks: 199 us; 4 pairs and 2 rows 214, 1 block 212.
+// forward: 8 pairs per lane, 1 row at a time, rings of 4, 2 blocks per SM: 121 us; rings of 8
+//   126, 2 rows side by side and rings of 6 121 (but 24 + 8 heads, 4 x 8192: 105 against 95 us),
+//   3 blocks 181, 1 block 164, 4 pairs per lane 158 (more shuffles and addresses per byte);
+// backward: 8 pairs, 1 row, rings of 4, 2 blocks: 198 us; 2 rows 340 (128 registers are too few), 1 block 212,
+//   4 pairs and 4 rows 290.
 // rotation (2 x 23400 tokens, 24 heads of 128): 4 pairs, 4 rows, 4 blocks: 91 us; 8 pairs 93, 2 rows 99.
-constexpr int kFwdV = 8, kFwdRows = 2, kFwdDepth = 6, kFwdPerSm = 2;
+constexpr int kFwdV = 8, kFwdRows = 1, kFwdDepth = 4, kFwdPerSm = 2;
 constexpr int kBwdV = 8, kBwdRows = 1, kBwdDepth = 4, kBwdPerSm = 2;
 constexpr int kRotV = 4, kRotRows = 4, kRotPerSm = 4;
 constexpr int kFwdBlocks = kSms * kFwdPerSm;
 constexpr int kBwdBlocks = kSms * kBwdPerSm;  // each with a partial of dw
-constexpr int kAngleRows = 4;  // an item's angles cost about as much as this many rows
+// an item's angles cost about as much as this many rows: with 3 the call above takes 129 us, with 5 117,
+// but 24 + 8 heads 95 and 99, 12 + 3 heads of 80 94 and 98
+constexpr int kAngleRows = 4;
 
 struct Rows {
   const void* x; Strides3 xs;
