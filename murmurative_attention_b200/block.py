@@ -1,5 +1,5 @@
-"""A pre-norm block around ``slot_murmurate``: every product, norm and rotation between the two
-residual additions runs on this library's kernels.
+"""A pre-norm block around ``slot_murmurate``: every matrix product, residual addition, query norm and
+rotation runs on this library's kernels (the norms over the model's width are torch's).
 
     x = x + o_proj(slot_murmurate(rotated, normed q_proj(norm(x))))
     x = x + down(act(up(norm(x))))

@@ -132,22 +132,26 @@ __global__ void __launch_bounds__(kDzThreads, 3)
   }
 }
 
+// out[n] = the chunks' sums of column n: a warp takes every 32nd chunk of 32 neighbouring columns, then
+// a column's 32 sums go to the lanes of one warp.
 template <typename T>
-__global__ void __launch_bounds__(256) k_col_sum(const float* part, int chunks, int N, T* out) {
-  __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) k_col_sum(const float* part, int chunks, int N, T* out) {
+  __shared__ float s[32][33];
   sm100::pdl_wait();
   sm100::pdl_trigger();
-  const int n = blockIdx.x * 32 + (threadIdx.x & 31), ty = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = blockIdx.x * 32 + lane;
   float sum = 0.f;
-  if (n < N)
-    for (int c = ty; c < chunks; c += 8) sum += part[(int64_t)c * N + n];
-  s[ty][threadIdx.x & 31] = sum;
-  __syncthreads();
-  if (ty == 0 && n < N) {
-    sum = 0.f;
-    for (int r = 0; r < 8; ++r) sum += s[r][threadIdx.x];
-    Elem<T>::store(out + n, sum);
+  if (n < N) {
+#pragma unroll 4
+    for (int c = warp; c < chunks; c += 32) sum += part[(int64_t)c * N + n];
   }
+  s[warp][lane] = sum;
+  __syncthreads();
+  sum = s[lane][warp];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0 && blockIdx.x * 32 + warp < N) Elem<T>::store(out + blockIdx.x * 32 + warp, sum);
 }
 
 template <typename T, int V>
@@ -156,10 +160,18 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
   int cols = 32;
   while (cols < kDzThreads && cols * V < N) cols *= 2;
   const int blocks_x = (N + cols * V - 1) / (cols * V);
-  // six blocks per SM, so that the last ones leave little idle; at least 32 rows per chunk
-  int most = (148 * 6 + blocks_x - 1) / blocks_x;
+  // Two rounds of three blocks per SM, so that the last ones leave little idle. With slopes one round
+  // where two would leave a thread less than 64 rows, and 24 rows per chunk at least (bf16 8192 x 4096,
+  // gradients of 64 inputs with it: one round of 37 rows 70 us, 32 rows in 1.15 rounds 78; 4096 x 1024:
+  // chunks of 24 rows 18.2, of 32 19.1, of 48 20.6). Without them, half the bytes, 32 rows and two rounds
+  // (8192 x 4096: 42.0, one round 43.5).
+  const bool slopes = a.activation != MURM_ACT_NONE;
+  const int wave = 148 * 3 / blocks_x, least = slopes ? 24 : 32;
+  int most = 2 * wave;
+  if (slopes && (int64_t)most * 64 * (kDzThreads / cols) > M) most = wave;
+  if (most < 1) most = 1;
   if (most > kDzChunks) most = kDzChunks;
-  if (most > (M + 31) / 32) most = (M + 31) / 32;
+  if (most > (M + least - 1) / least) most = (M + least - 1) / least;
   // few rows per thread in all: one chunk, whose block writes db itself (a launch less)
   if (M <= 16 * (kDzThreads / cols)) most = 1;
   const int chunk = (M + most - 1) / most;
@@ -175,7 +187,7 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
     MURM_LAUNCH_PDL("linear_dz", (k_dz<T, V, true>), grid, kDzThreads, 0, st, dy, a.go_stride,
                 static_cast<const Slope<T>*>(a.slope), M, N, cols, chunk, dz, part, db);
   if (part)
-    MURM_LAUNCH_PDL("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 256, 0, st, (const float*)part, chunks, N,
+    MURM_LAUNCH_PDL("linear_col_sum", k_col_sum<T>, (N + 31) / 32, 1024, 0, st, (const float*)part, chunks, N,
                 static_cast<T*>(a.grad_bias));
 }
 
