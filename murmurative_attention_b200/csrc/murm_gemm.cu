@@ -253,17 +253,23 @@ __device__ __forceinline__ void put_rows(uint32_t buf, int lane, const uint4 (&v
 #pragma unroll
   for (int i = 0; i < 4; ++i) sts128(buf + chunk_at(i * 8 + (lane >> 2), lane & 3), v[i]);
 }
-// The same rows where 16-byte accesses are not aligned: element by element, columns side by side.
+// The same rows where 16-byte accesses are not aligned: element by element, columns side by side. Global
+// reads go out four together, rows past the last from that one (777 x 1001 -> 1111 bf16 with a residual:
+// 21.0 us one by one, 19.6 so, 17.8 eight together, which spills: 8192 x 1024 -> 4096 63 us for 61.8).
 template <typename T, bool STORE>
 __device__ __forceinline__ void copy_rows(uint8_t* buf, T* g, int64_t ld, int rows, int cols, int lane) {
   constexpr int kCols = Out<T>::kCols, kRows = 32 / kCols;  // columns of a row, rows side by side
   const int c = lane % kCols;
   if (c >= cols) return;
-  for (int r = lane / kCols; r < rows; r += kRows) {
-    T* s = reinterpret_cast<T*>(buf + chunk_at(r, (c * (int)sizeof(T)) >> 4) + ((c * (int)sizeof(T)) & 15));
-    if (STORE) g[r * ld + c] = *s;
-    else *s = g[r * ld + c];
+  auto at = [&](int r) {
+    return reinterpret_cast<T*>(buf + chunk_at(r, (c * (int)sizeof(T)) >> 4) + ((c * (int)sizeof(T)) & 15));
+  };
+  if (STORE) {
+    for (int r = lane / kCols; r < rows; r += kRows) g[r * ld + c] = *at(r);
+    return;
   }
+#pragma unroll 4
+  for (int r = lane / kCols; r < 32; r += kRows) *at(r) = __ldg(g + min(r, rows - 1) * ld + c);
 }
 // The bias of a step's columns: the same address in every lane, from L1. With `vec`, b holds it
 // (loaded early, while the accumulator is on its way).
@@ -573,7 +579,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 2) tmem_free_pair(tmem, L::kTmemCols);
 }
 
-// out = epilogue of the K splits' sums, added in order. Four columns per thread.
+// out = epilogue of the K splits' sums, added in order. Four columns per thread; bias and residual are
+// read first, beside the sums, at clamped columns (2048 x 1024 -> 1024 fp32 with both: 35.9 us, 38.0 where
+// they were read one by one between the stores).
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_split_sum(const float* part, int64_t split_stride, int ldp, const __grid_constant__ Args p) {
@@ -582,6 +590,15 @@ __global__ void __launch_bounds__(256)
   const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
   const int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
   if (n >= p.N || m >= p.M) return;
+  float b[4] = {}, r[4] = {};
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = Elem<T>::load(static_cast<const T*>(p.bias) + min(n + j, p.N - 1));
+  }
+  if (p.res) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = Elem<T>::load(static_cast<const T*>(p.res) + m * p.ldr + min(n + j, p.N - 1));
+  }
   const float* src = part + m * ldp + n;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < p.splits; i += 4) {  // four splits' loads together, added in order
@@ -599,10 +616,9 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (n + j >= p.N) break;
-    if (p.bias) z[j] += Elem<T>::load(static_cast<const T*>(p.bias) + n + j);
-    float slope, y = act_value<Out<T>::kFast>(z[j], p.act, slope);
+    float slope;
+    const float y = act_value<Out<T>::kFast>(z[j] + b[j], p.act, slope) + r[j];
     if (p.slope) Elem<Slope<T>>::store(static_cast<Slope<T>*>(p.slope) + m * p.N + n + j, slope);
-    if (p.res) y += Elem<T>::load(static_cast<const T*>(p.res) + m * p.ldr + n + j);
     Elem<T>::store(static_cast<T*>(p.out) + m * p.ldo + n + j, y);
   }
 }
@@ -644,7 +660,10 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackArgs a
         *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(s + 4);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? s[e] : 0.f;
+        for (int e = 0; e < 8; ++e) v[e] = s[min(e, p.cols - 1 - c)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e >= p.cols) v[e] = 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -657,7 +676,10 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackArgs a
         *reinterpret_cast<uint4*>(dst + q * p.plane) = *reinterpret_cast<const uint4*>(o[q]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[0][e] = c + e < p.cols ? *reinterpret_cast<const uint16_t*>(s + e) : 0;
+      for (int e = 0; e < 8; ++e) o[0][e] = *reinterpret_cast<const uint16_t*>(s + min(e, p.cols - 1 - c));
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e >= p.cols) o[0][e] = 0;
       *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o[0]);
     }
   }
