@@ -135,6 +135,30 @@ def test_every_row_count(dtype):
         check(x, w, b, r, None, "silu", fused_linear(x, w, b, activation="silu", residual=r), None)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n,pad", [(263, 131, 0), (264, 200, 3), (1030, 1, 0), (17, 515, 2)])
+def test_every_row_count_without_alignment(dtype, k, n, pad):
+    """Rows that are not 16-byte aligned, one output, fewer columns than a warp's share."""
+    g = torch.Generator().manual_seed(7)
+    w, b = make((n, k), dtype, g, k ** -0.5, pad), make((1, n), dtype, g)[0]
+    for m in list(range(1, 20)) + [31, 32, 33, 48, 49, 80, 100, 128, 300]:
+        x, r = make((m, k), dtype, g, 1.0, pad), make((m, n), dtype, g, 1.0, pad)
+        check(x, w, b, r, None, "gelu", fused_linear(x, w, b, activation="gelu", residual=r), None)
+
+
+def test_last_columns_of_a_row_may_be_special():
+    """An infinity or NaN beside an odd row's end stays out of it; one in its last column counts."""
+    for dtype in DTYPES:
+        wide = torch.ones(3, 40, device="cuda", dtype=dtype)
+        wide[:, 33:] = float("nan")
+        w = torch.ones(5, 33, device="cuda", dtype=dtype)
+        assert bool((fused_linear(wide[:, :33], w) == 33).all())
+        x = torch.ones(3, 33, device="cuda", dtype=dtype)
+        x[1, 32] = float("inf")
+        got = fused_linear(x, w)
+        assert bool((got[0] == 33).all()) and bool((got[2] == 33).all()) and not bool(got[1].isfinite().any())
+
+
 def test_fp32_keeps_fp32_accuracy():
     """Terms of one sign, values with full mantissas and of mixed magnitudes."""
     g = torch.Generator().manual_seed(8)
