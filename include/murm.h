@@ -424,9 +424,10 @@ MURM_API size_t murm_norm_rope_workspace(void);
  * with unit inner stride and the given row strides (any element alignment),
  * residual and out [rows, out_features] likewise, bias [out_features]. Sums
  * are in fp32 (fp32 inputs: exact three-term bf16 splits, fp32 accuracy).
- * slope, when not NULL, receives act'(z) ([rows, out_features] contiguous; fp16
- * beside 16-bit tensors, fp32 beside fp32) for the backward; it is needed
- * there unless the activation is MURM_ACT_NONE, which writes none.
+ * slope, when not NULL, receives act'(z) ([rows, out_features] contiguous; fp32
+ * beside fp32, beside 16-bit tensors uint16 codes c of (c - 8192) / 32768 with
+ * 65535 for NaN) for the backward; it is needed there unless the activation is
+ * MURM_ACT_NONE, which writes none.
  *
  * Backward: dz = grad_out * slope, rounded once to `dtype` where it becomes a
  * matrix operand; grad_x = dz W, grad_weight = dz^T x, grad_bias = column sums of

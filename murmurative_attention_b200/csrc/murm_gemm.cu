@@ -186,6 +186,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t pack2(float a, float b, const SlopeCode*) {
+  return __byte_perm(slope_bits(a), slope_bits(b), 0x5410);
+}
 __device__ __forceinline__ float2 unpack2(uint32_t u, const __half*) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
@@ -618,7 +621,7 @@ __global__ void __launch_bounds__(256)
     if (n + j >= p.N) break;
     float slope;
     const float y = act_value<Out<T>::kFast>(z[j] + b[j], p.act, slope) + r[j];
-    if (p.slope) Elem<Slope<T>>::store(static_cast<Slope<T>*>(p.slope) + m * p.N + n + j, slope);
+    if (p.slope) store_slope(static_cast<Slope<T>*>(p.slope) + m * p.N + n + j, slope);
     Elem<T>::store(static_cast<T*>(p.out) + m * p.ldo + n + j, y);
   }
 }

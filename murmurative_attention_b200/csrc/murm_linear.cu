@@ -83,11 +83,12 @@ __global__ void __launch_bounds__(kDzThreads, 3)
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
   auto row = [&](int r, const P& g, const PS& sl) {
-    float d[V];
+    float d[V], s[V];
+    if (SLOPE) load_slopes<V>(sl.e, s);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       d[e] = Elem<T>::load(g.e + e);
-      if (SLOPE) d[e] *= Elem<Slope<T>>::load(sl.e + e);
+      if (SLOPE) d[e] *= s[e];
       acc[e] += d[e];
     }
     if (SLOPE && dz.p) store_operand<T, V>(dz, (int64_t)r * dz.ld + n, d);

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_rows(const __grid_constant__ Ro
   float z = acc[0];
   if (p.bias) z += Elem<T>::load(static_cast<const T*>(p.bias) + n);
   float slope, y = act_value<sizeof(T) == 2>(z, p.act, slope);
-  if (p.slope) Elem<Slope<T>>::store(static_cast<Slope<T>*>(p.slope) + (int64_t)m * p.N + n, slope);
+  if (p.slope) store_slope(static_cast<Slope<T>*>(p.slope) + (int64_t)m * p.N + n, slope);
   if (p.res) y += Elem<T>::load(static_cast<const T*>(p.res) + (int64_t)m * p.ldr + n);
   Elem<T>::store(static_cast<T*>(p.out) + m * p.ldo + n, y);
 }

@@ -122,7 +122,7 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x_, const Tensor& weight_
   const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
   Tensor out = at::empty({M, N}, x.options()), slope;
   if (save && act != MURM_ACT_NONE)
-    slope = at::empty({M, N}, x.options().dtype(x.scalar_type() == at::kFloat ? at::kFloat : at::kHalf));
+    slope = at::empty({M, N}, x.options().dtype(x.scalar_type() == at::kFloat ? at::kFloat : at::kShort));
   if (M == 0) return {out, slope};
   Tensor bias, residual;
   murm_linear_args a{};

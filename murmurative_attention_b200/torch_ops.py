@@ -279,7 +279,7 @@ def _linear_fwd_fake(x, weight, bias, activation, residual):
     out = x.new_empty(x.shape[0], weight.shape[0])
     if activation == "none":
         return out, x.new_empty(0)
-    return out, torch.empty_like(out, dtype=torch.float32 if x.dtype == torch.float32 else torch.float16)
+    return out, torch.empty_like(out, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
 
 
 @torch.library.impl(_q("fused_linear_bwd"), "CUDA", lib=_LIB)

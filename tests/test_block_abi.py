@@ -55,8 +55,8 @@ def test_linear_argument_checks(kw, status):
 def test_linear_workspaces():
     lib = _lib.load_library()
     assert _linear()[1] == 0                                     # few rows, read in place
-    assert _linear(x=4098, rows=300)[1] >= 300 * 64 * 2          # a copy TMA can address
-    assert _linear(dtype=_lib.MURM_F32, rows=300)[1] >= 3 * 2 * (300 + 32) * 64  # three planes of both operands
+    assert _linear(x=4098, rows=30000)[1] >= 30000 * 64 * 2      # a copy TMA can address
+    assert _linear(dtype=_lib.MURM_F32, rows=30000)[1] >= 3 * 2 * (30000 + 32) * 64  # three planes of both operands
     b = _lib.LinearBwdArgs(300, 64, 32, _lib.MURM_F16, 1, 4096, 64, 8192, 64, 16384, 32768, 32, 65536, 64, 131072, 64,
                            262144)
     n = ctypes.c_size_t(0)
