@@ -179,17 +179,21 @@ void forward(const murm_linear_args& a, const RowsArgs& p, cudaStream_t st) {
 
 // Up to 8 rows, and up to 16 of fp32 (the tensor path's three planes and their packing cost more); more
 // rows, in groups of 16, as long as the groups' passes over W stay short: past that every warp's reads
-// of 16 rows of x bind. A pass over few columns costs what 256 do. Measured, these kernels / the tensor
-// cores, us:
+// of 16 rows of x bind. A pass over few columns costs what 256 do, and the tensor path less with a short
+// K. Measured, these kernels / the tensor cores, us:
 //   bf16 4 x 1024 -> 1024 2.6 / 8.4, 16 x 1024 -> 1024 4.1 / 9.9, 32 rows 7.4 / 10.0, 64 rows 11.5 / 10.1;
-//   128 x 256 -> 256 4.4 / 7.1; 8 x 4096 -> 4096 11.6 / 14.8, 16 rows 28 / 14.8;
+//   128 x 256 -> 256 4.0 / 6.6, 500 rows 9.2 / 6.6; 8000 x 64 -> 16 9.1 / 4.5, 800 x 2560 -> 16 5.9 / 9.2;
+//   8 x 4096 -> 4096 11.6 / 14.8, 16 rows 28 / 14.8;
 //   fp32 48 x 1024 -> 1024 11.7 / 17.3, 64 x 512 -> 2048 17.1 / 15.4;
 // where rows are not 16-byte aligned (the tensor path lays them out first):
 //   bf16 16 x 1001 -> 1111 7.7 / 16.0, 48 rows 20 / 17.8; 32 x 513 -> 2047 17.8 / 16.3;
 //   fp32 16 x 4095 -> 1023 19.4 / 27, 32 x 1001 -> 1111 12.6 / 17.8, 64 rows 19.4 / 18.3.
 bool few_rows(const murm_linear_args& a) {
   const bool f32 = a.dtype == MURM_F32;
-  const int64_t most = vectors(a) ? (f32 ? 3 << 20 : 2 << 20) : f32 ? 2 << 20 : 3 << 19;
+  const int64_t unit = f32 ? 1 << 20 : 1 << 19, by_k = unit + unit * a.in_features / 256;
+  const int64_t cap = (f32 ? 3 : 4) * unit;
+  int64_t most = by_k < cap ? by_k : cap;
+  if (!vectors(a)) most -= most / 4;
   const int64_t passes = (a.rows + 15) / 16 * a.out_features * (a.in_features < 256 ? 256 : a.in_features);
   return a.rows <= (f32 ? 16 : 8) || passes <= most;
 }
