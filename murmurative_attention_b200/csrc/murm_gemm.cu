@@ -15,11 +15,12 @@
 // result's rows are not 16-byte aligned).
 //
 // fp32 operands are three bf16 planes; the products of planes (i, j) with i + j <= 2 carry them to
-// 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K
-// split K; the parts' fp32 sums go to the workspace and k_split_sum adds them in order and runs the
+// 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K, and
+// fp32 ones of a long K, split K; the parts' fp32 sums go to the workspace and k_split_sum adds them in order and runs the
 // epilogue.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdio>
 
 #include "murm_linear.cuh"
@@ -63,7 +64,7 @@ static_assert(sizeof(Bars) <= 256, "barrier area");
 
 struct Args {
   int M, N;
-  int kblocks, iters, total, splits;      // stages per plane pair, per split, in all; K splits
+  int iters, total, splits;               // stages per split, in all; K splits
   int tiles_m, tiles_n, tiles, items;     // items: tiles * splits
   uint32_t idesc;
   int a_mn, b_mn;
@@ -92,6 +93,7 @@ struct Launch {
 static_assert(sizeof(Launch) <= 4000, "kernel parameters");
 
 // Plane pairs of an fp32 product, smallest terms first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0).
+constexpr int kPlanePairs = 6;
 __device__ __forceinline__ int plane_a(int pair) { return (0x021010 >> (4 * (5 - pair))) & 15; }
 __device__ __forceinline__ int plane_b(int pair) { return (0x201100 >> (4 * (5 - pair))) & 15; }
 
@@ -402,13 +404,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (t.which < 0) continue;
       const Problem& pr = l.q[TWO ? t.which : 0];
       const CUtensorMap *map_a = &pr.a, *map_b = &pr.b;
-      const int a_mn = pr.p.a_mn, b_mn = pr.p.b_mn, fp32 = pr.p.fp32, kblocks = pr.p.kblocks;
+      const int a_mn = pr.p.a_mn, b_mn = pr.p.b_mn, fp32 = pr.p.fp32;
+      // fp32: a part of K goes through all plane pairs, `per` stages each
+      const int per = fp32 ? (t.i1 - t.i0) / kPlanePairs : 0, k0 = fp32 ? t.i0 / kPlanePairs : t.i0;
       const int ma = t.m0 + (int)rank * 128, nb = t.n0 + (int)rank * (BN / 2);
       const int skip = (mine + kLoaders - base % kLoaders) % kLoaders;
       int s = (base + skip) % L::kStages;
       uint32_t ph = ((base + skip) / L::kStages) & 1;  // the parity of the stage's round
-      int pair = fp32 ? (t.i0 + skip) / kblocks : 0;
-      int kb = t.i0 + skip - pair * kblocks;
+      int pair = fp32 ? skip / per : 0;
+      int kb = k0 + skip - pair * per;
       for (int i = t.i0 + skip; i < t.i1; i += kLoaders) {
         if (!(ok = wait(&bars->empty[s], ph ^ 1))) break;
         if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
@@ -429,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tma_load_pair(sb, map_b, k, nb, pb, bar);
         }
         kb += kLoaders;
-        while (fp32 && kb >= kblocks) { kb -= kblocks; ++pair; }
+        while (fp32 && kb >= k0 + per) { kb -= per; ++pair; }
         s += kLoaders;
         if (s >= L::kStages) { s -= L::kStages; ph ^= 1; }
       }
@@ -590,8 +594,8 @@ __global__ void __launch_bounds__(256)
     k_split_sum(const float* part, int64_t split_stride, int ldp, const __grid_constant__ Args p) {
   pdl_wait();
   pdl_trigger();
-  const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
-  const int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int n = (blockIdx.y * 64 + (threadIdx.x & 63)) * 4;
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= p.N || m >= p.M) return;
   float b[4] = {}, r[4] = {};
   if (p.bias) {
@@ -699,14 +703,14 @@ bool tma_rows(const void* p, int64_t ld, size_t es) {
 int64_t pitch_of(int cols) { return ((int64_t)cols + 7) / 8 * 8; }
 
 struct Config {
-  int bn, splits, iters, total, kblocks, tiles_m, tiles_n;
+  int bn, splits, iters, total, tiles_m, tiles_n;
 };
 
 Config config(const Gemm& g, int bn, int splits) {
-  const int kblocks = (g.K + kBK - 1) / kBK;
-  const int total = kblocks * (g.a.planes == 3 ? 6 : 1);
-  const int iters = (total + splits - 1) / splits;
-  return Config{bn, (total + iters - 1) / iters, iters, total, kblocks, (g.M + 255) / 256, (g.N + bn - 1) / bn};
+  const int kblocks = (g.K + kBK - 1) / kBK, pairs = g.a.planes == 3 ? kPlanePairs : 1;
+  const int total = kblocks * pairs;
+  const int iters = (kblocks + splits - 1) / splits * pairs;
+  return Config{bn, (total + iters - 1) / iters, iters, total, (g.M + 255) / 256, (g.N + bn - 1) / bn};
 }
 
 // Tile width and K splits by estimated time, in microseconds measured on B200:
@@ -725,12 +729,21 @@ double split_us(const Config& c) {
 bool split_fits(const Config& c, int splits) {
   return splits == 1 || (c.total / splits >= 2 && (int64_t)c.tiles_m * c.tiles_n * splits <= 2 * kPairs);
 }
+// The tensor cores cut each partial sum to 24 bits. So that fp32 keeps its accuracy, no accumulator
+// takes more than 1024 of K (16 parts at most, and as long as their sums fit 4 GB): 955 x 2064 -> 3224
+// has an error of 7.0e-7 of its norm in 97 us, 2.2e-6 in 79 with parts by time alone (a plain fp32
+// product 8.1e-7); 4096^3 1.1e-6 in 638 us, 4.5e-6 in 613 (1.2e-6).
+int least_splits(const Gemm& g) {
+  if (g.a.planes != 3) return 1;
+  const int parts = std::min((g.K + 1023) / 1024, 16);
+  return (int64_t)(g.M + 255) / 256 * ((g.N + 255) / 256) * parts <= (1 << 14) ? parts : 1;
+}
 double choose_one(const Gemm& g, Config* best) {
   double best_t = 0;
   for (int bn : {256, 128})
-    for (int splits = 1; splits <= 16; ++splits) {
+    for (int splits = least_splits(g), least = splits; splits <= 16; ++splits) {
       const Config c = config(g, bn, splits);
-      if (!split_fits(c, splits)) break;
+      if (splits > least && !split_fits(c, splits)) break;
       const int64_t rounds = ((int64_t)c.tiles_m * c.tiles_n * c.splits + kPairs - 1) / kPairs;
       const double t = rounds * c.iters * stage_us(bn) + split_us(c);
       if (best_t == 0 || t < best_t) {
@@ -767,7 +780,8 @@ Plan choose(const Gemm* g, int count) {
       for (int splits : kSplits) {
         Option& o = opt[i][n[i]];
         o.c = config(g[i], bn, splits);
-        if (!split_fits(o.c, splits)) break;
+        if (splits < least_splits(g[i])) continue;
+        if (n[i] && !split_fits(o.c, splits)) break;
         o.item = o.c.iters * stage_us(bn);
         o.work = o.item * o.c.tiles_m * o.c.tiles_n * o.c.splits;
         o.extra = split_us(o.c);
@@ -854,7 +868,7 @@ CUresult describe(const Gemm& g, const Config& c, void* workspace, Problem* q) {
   Args& p = q->p;
   p = Args{};
   p.M = g.M; p.N = g.N;
-  p.kblocks = c.kblocks; p.iters = c.iters; p.total = c.total; p.splits = c.splits;
+  p.iters = c.iters; p.total = c.total; p.splits = c.splits;
   p.tiles_m = c.tiles_m;
   p.tiles_n = c.tiles_n;
   p.tiles = c.tiles_m * c.tiles_n;
@@ -937,7 +951,7 @@ murm_status launch_tc(const Gemm* g, const Config* c, int count, char* workspace
     p.res = g[i].res; p.ldr = g[i].ldr;
     p.out = g[i].out; p.ldo = g[i].ldo;
     p.slope = g[i].slope;
-    launch("linear_split_sum", k_split_sum<T>, dim3((p.N + 255) / 256, (p.M + 3) / 4), 256, 0, st,
+    launch("linear_split_sum", k_split_sum<T>, dim3((p.M + 3) / 4, (p.N + 255) / 256), 256, 0, st,
            const_cast<const float*>(part[i]), stride, ldp, p);
   }
   const cudaError_t e = cudaGetLastError();

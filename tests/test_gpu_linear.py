@@ -135,6 +135,20 @@ def test_every_row_count(dtype):
         check(x, w, b, r, None, "silu", fused_linear(x, w, b, activation="silu", residual=r), None)
 
 
+@pytest.mark.parametrize("m,k,n", [(955, 2064, 3224), (300, 4000, 520), (40, 9000, 130), (4200, 1100, 4100)])
+def test_fp32_long_sums(m, k, n):
+    """No running sum takes more than 1024 terms: E of such sums, added over the parts like independent
+    errors, is below E of one sum of 1024 terms for S over all of them; 64 bits within it everywhere and
+    2^-20 of the norm overall (a plain fp32 sum of this length loses about 2^-21)."""
+    g = torch.Generator().manual_seed(31)
+    x, w = make((m, k), torch.float32, g), make((n, k), torch.float32, g, k ** -0.5)
+    want = x.double() @ w.double().t()
+    got = fused_linear(x, w)
+    s = (x.double().square() @ w.double().square().t()).sqrt()
+    within(got, want, (1024 / 16 + 16 + k / 1024) * 2.0 ** -23 * 4 * s, torch.float32)
+    assert float((got.double() - want).norm() / want.norm()) <= 2.0 ** -20
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("k,n,pad", [(263, 131, 0), (264, 200, 3), (1030, 1, 0), (17, 515, 2)])
 def test_every_row_count_without_alignment(dtype, k, n, pad):
