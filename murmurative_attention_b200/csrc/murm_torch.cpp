@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <array>
+
 #include "murm.h"
 
 namespace {
@@ -71,6 +73,14 @@ int dtype_code(const Tensor& t, const char* name) {
 
 void same_device(const Tensor& t, const Tensor& x, const char* name) {
   TORCH_CHECK(t.device() == x.device(), name, " must be on ", x.device(), ", got ", t.device());
+}
+
+// t (if there is one) has x's dtype and device.
+void like(const Tensor& t, const Tensor& x, const char* name) {
+  if (!t.defined()) return;
+  TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " must have x's dtype ", x.scalar_type(), ", got ",
+                   t.scalar_type());
+  same_device(t, x, name);
 }
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -235,27 +245,28 @@ int64_t activation_code(const std::string& name) {
   TORCH_CHECK_VALUE(false, "activation must be one of none, relu, silu, gelu, gelu_tanh, got '", name, "'");
 }
 
-Tensor fused_linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias_, const std::string& activation,
-                    const optional<Tensor>& residual_) {
-  const int64_t act = activation_code(activation);
-  const Tensor bias = value(bias_);
-  Tensor residual = value(residual_);
+// The arguments of every entry, the registered operators' too: the kernels take pointers and x's and
+// the weight's sizes. The residual's shape is the entry's to check.
+void check_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual) {
   dtype_code(x, "x");
   TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1),
               "x must be [..., K] and weight [N, K], got ", x.sizes(), " and ", weight.sizes());
   const int64_t N = weight.size(0), K = weight.size(1);
   TORCH_CHECK(N >= 1 && K >= 1, "weight must not be empty, got ", weight.sizes());
-  auto same = [&](const Tensor& t, const char* name) {
-    if (!t.defined()) return;
-    TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " must have x's dtype ", x.scalar_type(), ", got ",
-                     t.scalar_type());
-    same_device(t, x, name);
-  };
-  same(weight, "weight");
-  same(bias, "bias");
-  same(residual, "residual");
+  like(weight, x, "weight");
+  like(bias, x, "bias");
+  like(residual, x, "residual");
   TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), "bias must be [N=", N, "], got ",
               bias.sizes());
+}
+
+Tensor fused_linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias_, const std::string& activation,
+                    const optional<Tensor>& residual_) {
+  const int64_t act = activation_code(activation);
+  const Tensor bias = value(bias_);
+  Tensor residual = value(residual_);
+  check_linear(x, weight, bias, residual);
+  const int64_t N = weight.size(0), K = weight.size(1);
   const bool flat = x.dim() == 2;
   auto shape = x.sizes().vec();
   shape.back() = N;
@@ -489,23 +500,26 @@ struct QkNormRopeBackward : public Node {
   std::string name() const override { return "QkNormRopeBackward"; }
 };
 
+// q and k of every entry.
+void check_qk(const Tensor& q, const Tensor& k) {
+  check_rows(q, "q");
+  if (!k.defined()) return;
+  check_rows(k, "k");
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "q and k must share a dtype, got ", q.scalar_type(), " and ",
+                   k.scalar_type());
+  same_device(k, q, "k");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3), "k must be [B=", q.size(0),
+              ", Hk, N=", q.size(2), ", d=", q.size(3), "], got ", k.sizes());
+}
+
 std::pair<Tensor, optional<Tensor>> qk_norm_rope(const Tensor& q, const optional<Tensor>& k_, const Tensor& positions,
                                                  const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
                                                  double eps, double base, optional<int64_t> rotary_dim, bool interleaved,
                                                  const optional<std::vector<int64_t>>& sections,
                                                  const std::string& spectrum, const optional<Tensor>& freqs) {
-  check_rows(q, "q");
   const Tensor k = value(k_);
-  if (k.defined()) {
-    check_rows(k, "k");
-    TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "q and k must share a dtype, got ", q.scalar_type(), " and ",
-                     k.scalar_type());
-    same_device(k, q, "k");
-    TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3), "k must be [B=", q.size(0),
-                ", Hk, N=", q.size(2), ", d=", q.size(3), "], got ", k.sizes());
-  } else {
-    TORCH_CHECK(!defined(k_weight), "k_weight given without k");
-  }
+  check_qk(q, k);
+  TORCH_CHECK(k.defined() || !defined(k_weight), "k_weight given without k");
   const Tensor qw = gain(q_weight, q, "q_weight"), kw = k.defined() ? gain(k_weight, k, "k_weight") : Tensor();
   Rotation r = make_rotation(q, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, eps);
   auto [oq, ok] = norm_rope_forward(q, k, qw, kw, r);
@@ -575,14 +589,37 @@ Tensor rotary(const Tensor& x, const Tensor& positions, double base, optional<in
 // ---------------------------------------------------------------------------
 Tensor or_empty(const Tensor& t, const Tensor& like) { return t.defined() ? t : at::empty({0}, like.options()); }
 
+void check_rows_2d(const Tensor& x) { TORCH_CHECK(x.dim() == 2, "x must be [M, K], got ", x.sizes()); }
+
 std::tuple<Tensor, Tensor> linear_fwd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
-                                      const std::string& activation, const optional<Tensor>& residual) {
-  auto [out, slope] = linear_forward(x, weight, value(bias), value(residual), activation_code(activation), true);
+                                      const std::string& activation, const optional<Tensor>& residual_) {
+  const int64_t act = activation_code(activation);
+  const Tensor residual = value(residual_);
+  check_linear(x, weight, value(bias), residual);
+  check_rows_2d(x);
+  TORCH_CHECK(!residual.defined() || (residual.dim() == 2 && residual.size(0) == x.size(0) &&
+                                      residual.size(1) == weight.size(0)),
+              "residual must be [M=", x.size(0), ", N=", weight.size(0), "], got ", residual.sizes());
+  auto [out, slope] = linear_forward(x, weight, value(bias), residual, act, true);
   return {out, or_empty(slope, x)};
 }
 std::tuple<Tensor, Tensor, Tensor> linear_bwd(const Tensor& go, const Tensor& x, const Tensor& weight,
                                               const Tensor& slope, const std::string& activation) {
-  return linear_backward(go, x, weight, slope.numel() ? slope : Tensor(), activation_code(activation), true, true, true);
+  const int64_t act = activation_code(activation);
+  check_linear(x, weight, Tensor(), go);
+  check_rows_2d(x);
+  const std::array<int64_t, 2> sizes{x.size(0), weight.size(0)};
+  const c10::IntArrayRef shape(sizes);
+  TORCH_CHECK(go.sizes() == shape, "grad_out must be ", shape, ", got ", go.sizes());
+  if (act != MURM_ACT_NONE) {
+    const at::ScalarType type = x.scalar_type() == at::kFloat ? at::kFloat : at::kShort;
+    TORCH_CHECK_TYPE(slope.scalar_type() == type, "slope must be ", type, " beside ", x.scalar_type(), ", got ",
+                     slope.scalar_type());
+    same_device(slope, x, "slope");
+    TORCH_CHECK(slope.sizes() == shape && slope.is_contiguous(), "slope must be contiguous and ", shape, ", got ",
+                slope.sizes());
+  }
+  return linear_backward(go, x, weight, act != MURM_ACT_NONE ? slope : Tensor(), act, true, true, true);
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> qk_bwd(const Tensor& gq, const Tensor& gk, const Tensor& q,
                                                   const optional<Tensor>& k_, const Tensor& positions,
@@ -591,6 +628,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_bwd(const Tensor& gq, const Tensor
                                                   bool interleaved, const optional<std::vector<int64_t>>& sections,
                                                   const std::string& spectrum, const optional<Tensor>& freqs) {
   const Tensor k = value(k_);
+  check_qk(q, k);
+  like(gq, q, "grad_q");
+  TORCH_CHECK(gq.sizes() == q.sizes(), "grad_q must be ", q.sizes(), ", got ", gq.sizes());
+  if (k.defined()) {
+    like(gk, k, "grad_k");
+    TORCH_CHECK(gk.sizes() == k.sizes(), "grad_k must be ", k.sizes(), ", got ", gk.sizes());
+  }
   const Tensor x[2] = {q, k};
   const Tensor w[2] = {gain(q_weight, q, "q_weight"), k.defined() ? gain(k_weight, k, "k_weight") : Tensor()};
   const Tensor go[2] = {gq, gk};

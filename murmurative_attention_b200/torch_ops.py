@@ -274,8 +274,47 @@ def _linear_fwd_cuda(x, weight, bias, activation, residual):
     return _native.binding().linear_fwd(x, weight, bias, activation, residual)
 
 
+_LINEAR_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+_ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh")
+
+
+def _refuse(bad: bool, message: str, kind=RuntimeError) -> None:
+    if bad:
+        raise kind(message)
+
+
+def _like(t: Optional[Tensor], x: Tensor, name: str) -> None:
+    if t is not None:
+        _refuse(t.dtype != x.dtype, f"{name} must have x's dtype {x.dtype}, got {t.dtype}", TypeError)
+        _refuse(t.device != x.device, f"{name} must be on {x.device}, got {t.device}")
+
+
+def _check_linear(x, weight, activation, bias=None):
+    """What the compiled binding refuses of the linear operators' arguments, for their fakes: a trace fails
+    where the call would."""
+    _refuse(activation not in _ACTIVATIONS, f"activation must be one of {', '.join(_ACTIVATIONS)}, got '{activation}'",
+            ValueError)
+    _refuse(x.dtype not in _LINEAR_DTYPES, f"x must be float32, float16 or bfloat16, got {x.dtype}", TypeError)
+    _refuse(x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1],
+            f"x must be [M, K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _refuse(weight.shape[0] < 1 or weight.shape[1] < 1, f"weight must not be empty, got {tuple(weight.shape)}")
+    _like(weight, x, "weight")
+    _like(bias, x, "bias")
+    _refuse(bias is not None and (bias.dim() != 1 or bias.shape[0] != weight.shape[0]),
+            f"bias must be [N={weight.shape[0]}], got {tuple(bias.shape) if bias is not None else None}")
+
+
+def _check_outputs(t: Tensor, x: Tensor, weight: Tensor, name: str) -> None:
+    _refuse(t.dim() != 2 or t.shape[0] != x.shape[0] or t.shape[1] != weight.shape[0],
+            f"{name} must be [M={x.shape[0]}, N={weight.shape[0]}], got {tuple(t.shape)}")
+
+
 @torch.library.register_fake(_q("fused_linear_fwd"), lib=_LIB)
 def _linear_fwd_fake(x, weight, bias, activation, residual):
+    _check_linear(x, weight, activation, bias)
+    if residual is not None:
+        _like(residual, x, "residual")
+        _check_outputs(residual, x, weight, "residual")
     out = x.new_empty(x.shape[0], weight.shape[0])
     if activation == "none":
         return out, x.new_empty(0)
@@ -289,6 +328,14 @@ def _linear_bwd_cuda(grad_out, x, weight, slope, activation):
 
 @torch.library.register_fake(_q("fused_linear_bwd"), lib=_LIB)
 def _linear_bwd_fake(grad_out, x, weight, slope, activation):
+    _check_linear(x, weight, activation)
+    _like(grad_out, x, "grad_out")
+    _check_outputs(grad_out, x, weight, "grad_out")
+    if activation != "none":
+        kind = torch.float32 if x.dtype == torch.float32 else torch.int16
+        _refuse(slope.dtype != kind, f"slope must be {kind} beside {x.dtype}, got {slope.dtype}", TypeError)
+        _refuse(slope.device != x.device, f"slope must be on {x.device}, got {slope.device}")
+        _check_outputs(slope, x, weight, "slope")
     return x.new_empty(x.shape), x.new_empty(weight.shape), x.new_empty(weight.shape[0])
 
 
@@ -311,6 +358,8 @@ torch.library.register_autograd(_q("fused_linear_fwd"), _linear_backward, setup_
 def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: str,
                  residual: Optional[Tensor]) -> Tensor:
     """The registered form of ``fused_linear`` (same operation; traceable by torch.compile)."""
+    _refuse(x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1],
+            f"x must be [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
     shape = x.shape[:-1] + (weight.shape[0],)
     x2 = x.reshape(-1, x.shape[-1])
     r2 = residual.expand(shape).reshape(-1, shape[-1]) if residual is not None else None
@@ -342,6 +391,10 @@ def _qk_bwd_cuda(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation)
 
 @torch.library.register_fake(_q("qk_norm_rope_bwd"), lib=_LIB)
 def _qk_bwd_fake(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation):
+    for g, t, name in ((grad_q, q, "grad_q"), (grad_k, k, "grad_k")):
+        if t is not None:
+            _like(g, t, name)
+            _refuse(g.shape != t.shape, f"{name} must be {tuple(t.shape)}, got {tuple(g.shape)}")
     none = q.new_empty(0)
     return (_unit_layout(q), _unit_layout(k) if k is not None else none,
             torch.empty_like(q_weight) if q_weight is not None else none,

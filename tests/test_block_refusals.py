@@ -1,0 +1,82 @@
+"""Refusals of the block operators without a GPU: fake CUDA tensors go through the compiled binding's
+checks (which raise before anything is allocated or launched) and through the registered operators' fakes,
+which have to refuse while tracing what the eager call refuses."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from murmurative_attention_b200 import _native, torch_ops
+
+NS = torch.ops.murmurative_attention
+
+
+@pytest.fixture
+def fake():
+    with FakeTensorMode():
+        yield lambda *shape, dtype=torch.bfloat16, device="cuda": torch.empty(shape, dtype=dtype, device=device)
+
+
+# x [4, 64], weight [32, 64] bf16 and one thing wrong
+LINEAR = [
+    (dict(weight=(32, 128)), RuntimeError), (dict(weight=(32, 32)), RuntimeError), (dict(weight=(64,)), RuntimeError),
+    (dict(weight=(32, 64), weight_dtype=torch.float32), TypeError), (dict(weight_device="cpu"), RuntimeError),
+    (dict(weight=(0, 64)), RuntimeError),
+    (dict(bias=(4,)), RuntimeError), (dict(bias=(1, 32)), RuntimeError), (dict(bias=(32,), bias_dtype=torch.float32), TypeError),
+    (dict(bias=(32,), bias_device="cpu"), RuntimeError),
+    (dict(residual=(3, 32)), RuntimeError), (dict(residual=(4, 31)), RuntimeError),
+    (dict(residual=(4, 32), residual_dtype=torch.float32), TypeError), (dict(residual=(4, 32), residual_device="cpu"), RuntimeError),
+    (dict(activation="swish"), ValueError), (dict(x_dtype=torch.float64, weight_dtype=torch.float64), TypeError),
+]
+
+
+def linear_args(fake, c):
+    make = lambda name, default: fake(*c.get(name, default), dtype=c.get(f"{name}_dtype", torch.bfloat16),
+                                      device=c.get(f"{name}_device", "cuda"))
+    return (make("x", (4, 64)), make("weight", (32, 64)), make("bias", ()) if "bias" in c else None,
+            c.get("activation", "gelu"), make("residual", ()) if "residual" in c else None)
+
+
+@pytest.mark.parametrize("case,error", LINEAR)
+def test_linear_refused_everywhere(fake, case, error):
+    args = linear_args(fake, case)
+    for call in (NS.fused_linear_fwd, torch_ops.fused_linear, _native.binding().fused_linear, _native.binding().linear_fwd):
+        with pytest.raises(error):
+            call(*args)
+
+
+@pytest.mark.parametrize("case,error", [
+    (dict(go=(4, 31)), RuntimeError), (dict(go=(3, 32)), RuntimeError), (dict(go_dtype=torch.float32), TypeError),
+    (dict(go_device="cpu"), RuntimeError), (dict(slope=(4, 31)), RuntimeError), (dict(slope=(0,)), RuntimeError),
+    (dict(slope_dtype=torch.bfloat16), TypeError), (dict(slope_device="cpu"), RuntimeError),
+    (dict(weight=(32, 128)), RuntimeError), (dict(weight_device="cpu"), RuntimeError), (dict(activation="swish"), ValueError),
+])
+def test_linear_gradients_refused(fake, case, error):
+    x, w, _, act, _ = linear_args(fake, case)
+    go = fake(*case.get("go", (4, 32)), dtype=case.get("go_dtype", torch.bfloat16), device=case.get("go_device", "cuda"))
+    slope = fake(*case.get("slope", (4, 32)), dtype=case.get("slope_dtype", torch.int16),
+                 device=case.get("slope_device", "cuda"))
+    for call in (NS.fused_linear_bwd, _native.binding().linear_bwd):
+        with pytest.raises(error):
+            call(go, x, w, slope, act)
+
+
+@pytest.mark.parametrize("case,error", [
+    (dict(gq=(1, 2, 4, 64)), RuntimeError), (dict(gq=(1, 2, 5, 32)), RuntimeError), (dict(gk=(1, 2, 5, 64)), RuntimeError),
+    (dict(gq_dtype=torch.float32), TypeError), (dict(gk_device="cpu"), RuntimeError),
+])
+def test_norm_rope_gradients_refused(fake, case, error):
+    q, k, pos = fake(1, 2, 5, 64), fake(1, 1, 5, 64), fake(5, dtype=torch.int64)
+    gq = fake(*case.get("gq", (1, 2, 5, 64)), dtype=case.get("gq_dtype", torch.bfloat16))
+    gk = fake(*case.get("gk", (1, 1, 5, 64)), device=case.get("gk_device", "cuda"))
+    rest = (None, None, 1e-6, 1e4, None, False, None, "shared", None)
+    for call in (NS.qk_norm_rope_bwd, _native.binding().qk_bwd):
+        with pytest.raises(error):
+            call(gq, gk, q, k, pos, *rest)
+
+
+def test_what_fits_is_traced(fake):
+    x, w, b, r = fake(4, 64), fake(32, 64), fake(32), fake(4, 32)
+    out, slope = NS.fused_linear_fwd(x, w, b, "gelu", r)
+    assert out.shape == slope.shape == (4, 32) and slope.dtype == torch.int16
+    assert [t.shape for t in NS.fused_linear_bwd(out, x, w, slope, "gelu")] == [(4, 64), (32, 64), (32,)]
+    assert torch_ops.fused_linear(fake(2, 3, 64), w, b, "none", fake(3, 32)).shape == (2, 3, 32)
