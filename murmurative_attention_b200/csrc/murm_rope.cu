@@ -502,14 +502,16 @@ template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(kThreads, kRotPerSm) k_rotate(const __grid_constant__ Params p) {
   constexpr int U = UnitsPerLane<V>::v, F = U == 1 ? kRotRows : 1, P = Pairs<V>::v;
   using R = Raw<T, V>;
-  const Rows& r = p.t[0];
+  const bool second = blockIdx.x >= p.t[0].blocks;
+  const Rows& r = p.t[second];
+  const int block = blockIdx.x - (second ? p.t[0].blocks : 0);
   const int groups = kThreads / p.L, group = threadIdx.x / p.L, lane = threadIdx.x - group * p.L;
   if (group >= groups) return;
   LaneState<T, V, INTER> st;
 #pragma unroll
   for (int j = 0; j < U; ++j) st.at[j] = unit_at<V, INTER>(p, lane + p.L * j);
   Walk w;
-  w.start(p, r, blockIdx.x * groups + group, 0);
+  w.start(p, r, block * groups + group, 0);
   const T* x = row_ptr(static_cast<const T*>(r.x), r.xs, w.b, w.c * r.chunk, w.n);
   T* y = row_ptr(static_cast<T*>(r.y), r.ys, w.b, w.c * r.chunk, w.n);
   R lo[F][U], hi[F][U];

@@ -1,0 +1,52 @@
+"""The block operators' C ABI on a GPU, where it takes more than the Python functions hand it."""
+import ctypes
+
+import pytest
+import torch
+
+from murmurative_attention_b200 import _lib, rotary
+
+pytestmark = pytest.mark.gpu
+CODES = {torch.float32: _lib.MURM_F32, torch.float16: _lib.MURM_F16, torch.bfloat16: _lib.MURM_BF16}
+NAN = float("nan")
+
+
+def set_rows(rows, x, out):
+    rows.x, rows.out, rows.heads = x.data_ptr(), out.data_ptr(), x.shape[1]
+    for i in range(3):
+        rows.x_stride[i], rows.out_stride[i] = x.stride(i), out.stride(i)
+
+
+def rope_args(x, pos, **kw):
+    B, _, N, d = x.shape
+    a = _lib.NormRopeArgs(batch=B, tokens=N, head_dim=d, rotary_dim=d, dtype=CODES[x.dtype], axes=1, eps=1e-6, base=1e4,
+                          position_type=_lib.MURM_POS_I64)
+    a.positions = pos.data_ptr() if pos is not None else None
+    a.position_stride[1] = 1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def run(a):
+    assert _lib.load_library().murm_norm_rope_fwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", list(CODES))
+@pytest.mark.parametrize("N,d", [(1, 64), (37, 72), (300, 128), (5, 10)])
+@pytest.mark.parametrize("hq,hk", [(4, 1), (3, 7), (0, 2), (2, 0)])
+def test_rotation_alone_takes_q_and_k(dtype, N, d, hq, hk):
+    """Without the norm, every row of q and k: bit for bit what each gives by itself, with either absent."""
+    g = torch.Generator().manual_seed(1)
+    q, k = (torch.randn(2, h, N, d, generator=g).to(dtype).cuda() for h in (hq, hk))
+    pos = torch.randint(0, 100000, (N,), generator=g).cuda()
+    oq, ok = torch.full_like(q, NAN), torch.full_like(k, NAN)
+    a = rope_args(q, pos)
+    if hq:
+        set_rows(a.q, q, oq)
+    if hk:
+        set_rows(a.k, k, ok)
+    run(a)
+    for x, o in ((q, oq), (k, ok)):
+        assert torch.equal(o, rotary(x, pos))
