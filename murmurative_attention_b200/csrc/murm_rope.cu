@@ -433,7 +433,7 @@ struct Ring {
   __device__ __forceinline__ void enter() {
     row[0] = row_ptr(static_cast<const T*>(r.x), r.xs, w.b, w.c * r.chunk, w.n);
     if (A == 2) row[A - 1] = row_ptr(static_cast<const T*>(r.g), r.gs, w.b, w.c * r.chunk, w.n);
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(w.position(p)));
+    if (p.rot_units) asm volatile("prefetch.global.L1 [%0];" ::"l"(w.position(p)));  // else there may be none
   }
   __device__ __forceinline__ void step() {
     if (w.template step<1>(p, r)) {

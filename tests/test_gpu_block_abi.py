@@ -50,3 +50,29 @@ def test_rotation_alone_takes_q_and_k(dtype, N, d, hq, hk):
     run(a)
     for x, o in ((q, oq), (k, ok)):
         assert torch.equal(o, rotary(x, pos))
+
+
+@pytest.mark.parametrize("dtype", list(CODES))
+def test_nothing_rotated_needs_no_positions(dtype):
+    """rotary_dim = 0: positions may be NULL, in the norm's forward and backward and in the rotation alone."""
+    lib, st = _lib.load_library(), torch.cuda.current_stream().cuda_stream
+    x = torch.randn(2, 3, 70, 64, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    zeros = torch.zeros(70, dtype=torch.int64, device="cuda")
+    res = []
+    for pos in (zeros, None):
+        out = torch.full_like(x, NAN)
+        a = rope_args(x, pos, normalize=1, rotary_dim=0)
+        set_rows(a.q, x, out)
+        run(a)
+        gx = torch.full_like(x, NAN)
+        set_rows(a.q, x, gx)
+        a.q.grad, a.q.grad_stride = x.data_ptr(), a.q.x_stride
+        assert lib.murm_norm_rope_bwd(ctypes.byref(a), st) == 0
+        torch.cuda.synchronize()
+        res.append((out, gx))
+    assert all(torch.equal(p, q) and bool(p.isfinite().all()) for p, q in zip(*res))
+    copy = torch.full_like(x, NAN)
+    a = rope_args(x, None, rotary_dim=0)
+    set_rows(a.q, x, copy)
+    run(a)
+    assert torch.equal(copy, x)
