@@ -812,6 +812,8 @@ murm_status check_rows(const murm_norm_rope_args& a, const murm_head_rows& r, co
       return bad(MURM_ERR_INVALID_ARGUMENT, "%s: out stride[%d] is zero", name, i);
   if ((r.weight || r.grad_weight) && r.weight_dtype != MURM_F32 && r.weight_dtype != a.dtype)
     return bad(MURM_ERR_DTYPE, "%s weight must be fp32 or of the rows' dtype, got code %d", name, r.weight_dtype);
+  if ((reinterpret_cast<uintptr_t>(r.weight) | reinterpret_cast<uintptr_t>(r.grad_weight)) % elem_size(r.weight_dtype))
+    return bad(MURM_ERR_INVALID_ARGUMENT, "%s: a weight pointer is not aligned to its element", name);
   const double rows = (double)a.batch * r.heads * a.tokens;
   if (rows > 2146435072.0) return bad(MURM_ERR_UNSUPPORTED, "%s: batch*heads*tokens exceeds 2^31 - 2^20 rows", name);
   return MURM_OK;
@@ -842,6 +844,9 @@ murm_status check_args(const murm_norm_rope_args* a, bool backward) {
     return bad(MURM_ERR_DTYPE, "unsupported position type code %d", a->position_type);
   if (a->rotary_dim > 0 && !a->positions && a->batch > 0 && a->tokens > 0)
     return bad(MURM_ERR_INVALID_ARGUMENT, "positions is NULL");
+  if (reinterpret_cast<uintptr_t>(a->positions) % (a->position_type == MURM_POS_I64 ? 8 : 4) ||
+      reinterpret_cast<uintptr_t>(a->freqs) % 4)
+    return bad(MURM_ERR_INVALID_ARGUMENT, "positions or freqs is not aligned to its element");
   if (!a->freqs && !(a->base > 0 && std::isfinite(a->base)))
     return bad(MURM_ERR_INVALID_ARGUMENT, "base must be positive and finite");
   if (a->normalize && !(a->eps >= 0 && std::isfinite(a->eps)))

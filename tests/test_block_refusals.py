@@ -1,11 +1,13 @@
 """Refusals of the block operators without a GPU: fake CUDA tensors go through the compiled binding's
 checks (which raise before anything is allocated or launched) and through the registered operators' fakes,
 which have to refuse while tracing what the eager call refuses."""
+import ctypes
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from murmurative_attention_b200 import _native, torch_ops
+from murmurative_attention_b200 import _lib, _native, torch_ops
 
 NS = torch.ops.murmurative_attention
 
@@ -80,3 +82,20 @@ def test_what_fits_is_traced(fake):
     assert out.shape == slope.shape == (4, 32) and slope.dtype == torch.int16
     assert [t.shape for t in NS.fused_linear_bwd(out, x, w, slope, "gelu")] == [(4, 64), (32, 64), (32,)]
     assert torch_ops.fused_linear(fake(2, 3, 64), w, b, "none", fake(3, 32)).shape == (2, 3, 32)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(), 0), (dict(positions=4100, position_type=_lib.MURM_POS_I32), 0),
+    (dict(positions=4100), 1), (dict(positions=4098, position_type=_lib.MURM_POS_F32), 1), (dict(freqs=4098), 1),
+    (dict(weight=4097), 1), (dict(weight=4098), 0), (dict(weight=4098, weight_dtype=_lib.MURM_F32), 1),
+])
+def test_norm_rope_pointers_are_aligned(kw, status):
+    """No batch: a call that passes the checks launches nothing."""
+    a = _lib.NormRopeArgs(batch=0, tokens=4, head_dim=64, rotary_dim=64, dtype=_lib.MURM_F16, normalize=1, axes=1,
+                          eps=1e-6, base=1e4, positions=4096)
+    a.q.heads, a.q.weight_dtype = 2, _lib.MURM_F16
+    for k, v in kw.items():
+        setattr(a.q if k.startswith("weight") else a, k, v)
+    if "freqs" in kw:
+        a.freqs = kw["freqs"]
+    assert _lib.load_library().murm_norm_rope_fwd(ctypes.byref(a), None) == status
