@@ -71,6 +71,8 @@ int dtype_code(const Tensor& t, const char* name) {
   }
 }
 
+constexpr int64_t kMaxSize = INT32_MAX;  // of what the C ABI takes in 32 bits, checked before it is cut to them
+
 void same_device(const Tensor& t, const Tensor& x, const char* name) {
   TORCH_CHECK(t.device() == x.device(), name, " must be on ", x.device(), ", got ", t.device());
 }
@@ -253,6 +255,7 @@ void check_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, con
               "x must be [..., K] and weight [N, K], got ", x.sizes(), " and ", weight.sizes());
   const int64_t N = weight.size(0), K = weight.size(1);
   TORCH_CHECK(N >= 1 && K >= 1, "weight must not be empty, got ", weight.sizes());
+  TORCH_CHECK(N <= kMaxSize && K <= kMaxSize, "features must be below 2^31, got ", weight.sizes());
   like(weight, x, "weight");
   like(bias, x, "bias");
   like(residual, x, "residual");
@@ -308,6 +311,7 @@ struct Rotation {
 void check_rows(const Tensor& t, const char* name) {
   dtype_code(t, name);
   TORCH_CHECK(t.dim() == 4, name, " must be 4-D [B, H, N, head_dim], got shape ", t.sizes());
+  for (const int64_t n : t.sizes()) TORCH_CHECK(n <= kMaxSize, name, "'s sizes must be below 2^31, got ", t.sizes());
 }
 
 Rotation make_rotation(const Tensor& x, const Tensor& positions, double base, optional<int64_t> rotary_dim,
@@ -362,7 +366,7 @@ Rotation make_rotation(const Tensor& x, const Tensor& positions, double base, op
     same_device(*freqs, x, "freqs");
     r.freqs = freqs->contiguous();
   }
-  a.head_dim = static_cast<int32_t>(std::min<int64_t>(d, INT32_MAX));
+  a.head_dim = static_cast<int32_t>(d);
   a.rotary_dim = static_cast<int32_t>(rd);
   a.interleaved = interleaved;
   a.own_spectrum = spectrum == "own";

@@ -99,3 +99,22 @@ def test_norm_rope_pointers_are_aligned(kw, status):
     if "freqs" in kw:
         a.freqs = kw["freqs"]
     assert _lib.load_library().murm_norm_rope_fwd(ctypes.byref(a), None) == status
+
+
+@pytest.mark.parametrize("big", [1 << 31, (1 << 32) + 8])
+def test_sizes_past_32_bits_are_refused(fake, big):
+    """They were cut to 32 bits: 2^32 + 8 features computed with 8."""
+    binding = _native.binding()
+    pos = fake(4, dtype=torch.int64)
+    for x, w in (((4, big), (3, big)), ((4, 8), (big, 8))):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            binding.fused_linear(fake(*x), fake(*w), None, "none", None)
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            binding.linear_fwd(fake(*x), fake(*w), None, "none", None)
+    for shape in ((big, 1, 4, 2), (1, big, 4, 2), (1, 1, big, 2), (1, 1, 4, big)):
+        rest = (1e4, None, False, None, "shared", None)
+        p = pos if shape[2] == 4 else fake(shape[2], dtype=torch.int64)
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            binding.rotary(fake(*shape), p, *rest, False)
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            binding.qk_norm_rope(fake(*shape), None, p, None, None, 1e-6, *rest)
