@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -94,6 +95,15 @@ Tensor bytes_on(const Tensor& like, size_t n) {
 bool defined(const optional<Tensor>& t) { return t.has_value() && t->defined(); }
 Tensor value(const optional<Tensor>& t) { return defined(t) ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// The operators run below the dispatcher, which neither forward-mode tangents nor torch.jit.trace see:
+// an output without its tangent, or an empty tensor in the traced graph, would pass for a result.
+template <typename... T>
+void refuse_unseen(const char* name, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!((inputs.defined() && inputs._fw_grad(0).defined()) || ...), name,
+                              " has no forward-mode derivative");
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be recorded by torch.jit.trace; torch.compile can");
+}
 
 // Gradients of a node that is differentiable once: differentiating them again raises.
 variable_list once(variable_list&& grads, const char* name) {
@@ -221,6 +231,7 @@ struct FusedLinearBackward : public Node {
     variable_list res(4);
     const Tensor& go = grads[0];
     if (!go.defined()) return res;
+    refuse_unseen("fused_linear's gradient", go);
     std::lock_guard<std::mutex> lock(mutex_);
     const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1),
                nb = task_should_compute_output(2);
@@ -269,6 +280,7 @@ Tensor fused_linear(const Tensor& x, const Tensor& weight, const optional<Tensor
   const Tensor bias = value(bias_);
   Tensor residual = value(residual_);
   check_linear(x, weight, bias, residual);
+  refuse_unseen("fused_linear", x, weight, bias, residual);
   const int64_t N = weight.size(0), K = weight.size(1);
   const bool flat = x.dim() == 2;
   auto shape = x.sizes().vec();
@@ -485,6 +497,7 @@ struct QkNormRopeBackward : public Node {
   Rotation r;  // without its tensors
 
   variable_list apply(variable_list&& grads) override {
+    for (const auto& go : grads) refuse_unseen("qk_norm_rope's gradient", go);
     std::lock_guard<std::mutex> lock(mutex_);
     Rotation now = r;
     now.positions = positions.unpack();
@@ -525,6 +538,7 @@ std::pair<Tensor, optional<Tensor>> qk_norm_rope(const Tensor& q, const optional
   check_qk(q, k);
   TORCH_CHECK(k.defined() || !defined(k_weight), "k_weight given without k");
   const Tensor qw = gain(q_weight, q, "q_weight"), kw = k.defined() ? gain(k_weight, k, "k_weight") : Tensor();
+  refuse_unseen("qk_norm_rope", q, k, qw, kw);
   Rotation r = make_rotation(q, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, eps);
   auto [oq, ok] = norm_rope_forward(q, k, qw, kw, r);
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw))) {
@@ -567,6 +581,7 @@ struct RotaryBackward : public Node {
 };
 
 Tensor rotary_apply(const Tensor& x, const Rotation& r, bool inverse) {
+  refuse_unseen("rotary", x);
   Tensor out = rotate(x, r, inverse);
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     auto node = make_node<RotaryBackward>();
