@@ -397,6 +397,12 @@ Tensor gain(const optional<Tensor>& w, const Tensor& x, const char* name) {
   return w->contiguous();
 }
 
+// A result for t's rows, in their layout. Overlapping rows (a sliding window: token and element both of
+// stride 1) have none to keep, and empty_like's guess may put the tokens innermost.
+Tensor empty_rows(const Tensor& t) {
+  Tensor out = at::empty_like(t);
+  return out.stride(3) == 1 ? out : at::empty_like(t, at::MemoryFormat::Contiguous);
+}
 Tensor unit_rows(const Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); }
 void set_strides(int64_t (&dst)[3], const Tensor& t) {
   for (int i = 0; i < 3; ++i) dst[i] = t.stride(i);
@@ -430,7 +436,7 @@ Tensor rotate(const Tensor& x_, const Rotation& r, bool inverse) {
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(x_.device());
   const Tensor x = unit_rows(x_);
-  Tensor out = at::empty_like(x);
+  Tensor out = empty_rows(x);
   if (x.numel()) {
     murm_norm_rope_args a = call_args(r, x, false, inverse);
     set_rows(a.q, x, out, Tensor());
@@ -444,7 +450,7 @@ std::pair<Tensor, Tensor> norm_rope_forward(const Tensor& q_, const Tensor& k_, 
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = unit_rows(q_), k = k_.defined() ? unit_rows(k_) : k_;
-  Tensor oq = at::empty_like(q), ok = k.defined() ? at::empty_like(k) : Tensor();
+  Tensor oq = empty_rows(q), ok = k.defined() ? empty_rows(k) : Tensor();
   if (q.numel() || (k.defined() && k.numel())) {
     murm_norm_rope_args a = call_args(r, q, true, false);
     set_rows(a.q, q, oq, qw);
@@ -466,7 +472,7 @@ variable_list norm_rope_backward(const Tensor (&x_)[2], const Tensor (&w)[2], co
   for (int t = 0; t < 2; ++t) {
     if (!x_[t].defined() || !need[t]) continue;
     x[t] = unit_rows(x_[t]);
-    gx[t] = at::empty_like(x[t]);
+    gx[t] = empty_rows(x[t]);
     if (x[t].numel() == 0) {  // no rows: gain gradients are sums of nothing
       if (w[t].defined()) gw[t] = at::zeros_like(w[t]);
       continue;

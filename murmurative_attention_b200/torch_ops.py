@@ -368,8 +368,10 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: 
 
 
 def _unit_layout(t: Tensor) -> Tensor:
-    """An empty tensor as the rotation's results are laid out: like the rows when their inner stride is 1."""
-    return torch.empty_like(t if t.stride(3) == 1 else t.contiguous())
+    """An empty tensor as the rotation's results are laid out: like the rows when their inner stride is 1
+    and the copy's is too (rows that overlap have no layout to keep)."""
+    out = torch.empty_like(t if t.stride(3) == 1 else t.contiguous())
+    return out if out.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 @torch.library.impl(_q("qk_norm_rope"), "CUDA", lib=_LIB)
