@@ -78,13 +78,18 @@ class MurmurativeBlock(nn.Module):
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, pool: SlotPool, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """One token per sequence, x [B, D]: select, attend and slot update on the pool, which advances.
+        """One token per sequence, x [B, D]: its ``rounds`` rounds of select, attend and slot update on the
+        pool, the attended values summed over them as in ``forward``; then the pool's positions advance. Tokens
+        so take all their rounds one after another, where ``forward`` runs each round over all tokens.
         positions: [B, 1] (with ``sections`` [B, 1, A]), by default the pool's."""
         if positions is None:
             if self.rope["sections"] is not None:
                 raise ValueError("positions of several axes have to be given")
             positions = pool.positions.unsqueeze(1)
         q = self._queries(self.norm1(x).unsqueeze(1), positions)[:, :, 0]
-        attn = pool.step(q, q, q, causal=self.causal, gamma=0.15)
+        attn = None if self.rounds else torch.zeros_like(q)
+        for _ in range(self.rounds):
+            attn = pool.step(q, q, q, attn, causal=self.causal, gamma=0.15, advance=False)
+        pool.positions += 1
         x = fused_linear(attn.reshape(x.shape), self.o_proj.weight, residual=x)
         return self._feed_forward(x)

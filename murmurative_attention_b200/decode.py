@@ -51,10 +51,11 @@ class SlotPool:
     @torch.no_grad()
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, x: Optional[torch.Tensor] = None,
              causal: bool = True, alpha: float = 0.9, gamma: float = 0.1, scale: Optional[float] = None,
-             return_selection: bool = False):
+             return_selection: bool = False, advance: bool = True):
         """One token per sequence: q, k, v (and the residual x) as [B, H, d] or [B, H*d].
         Returns x + attend in the input's layout (and (indices, weights) [B, H, 7] if
-        ``return_selection``); the pool and the positions advance in place."""
+        ``return_selection``); the pool and the positions advance in place (the positions not with
+        ``advance=False``: another round of the same token follows)."""
         B, H, M, D = self.keys.shape
         dt = self.keys.dtype
         flat = q.dim() == 2
@@ -74,6 +75,7 @@ class SlotPool:
             slot_values=_ptr(self.values), sv_stride=_lib.Strides(*self.values.stride()[:3]),
             indices=_ptr(idx), weights=_ptr(w))
         _lib.check(_lib.load_library().murm_decode_step(ctypes.byref(a), _stream()))
-        self.positions += 1
+        if advance:
+            self.positions += 1
         res = out.view(B, H * D) if flat else out
         return (res, idx, w) if return_selection else res
