@@ -15,9 +15,9 @@
 // result's rows are not 16-byte aligned).
 //
 // fp32 operands are three bf16 planes; the products of planes (i, j) with i + j <= 2 carry them to
-// 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K, and
-// fp32 ones of a long K, split K; the parts' fp32 sums go to the workspace and k_split_sum adds them in order and runs the
-// epilogue.
+// 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K split
+// K; the parts' fp32 sums go to the workspace and k_split_sum adds them in order and runs the epilogue. So
+// do fp32 products of a long K, whose items change accumulators on the way (kSegment).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -64,7 +64,7 @@ static_assert(sizeof(Bars) <= 256, "barrier area");
 
 struct Args {
   int M, N;
-  int iters, total, splits;               // stages per split, in all; K splits
+  int iters, total, splits, seg;          // stages per split, in all; K splits; stages per accumulator
   int tiles_m, tiles_n, tiles, items;     // items: tiles * splits
   uint32_t idesc;
   int a_mn, b_mn;
@@ -76,6 +76,7 @@ struct Args {
   void* slope; int slope_tma;
   int partial;     // out: fp32 sums of K splits, tiles side by side, splits `split_rows` rows apart
   int split_rows;
+  int join;        // an item's last segment reads what the earlier ones left in out, then runs the epilogue
 };
 struct Problem {
   CUtensorMap a, b, out, slope;
@@ -85,6 +86,7 @@ struct Problem {
 // `tabled` a position's item is order[position] (kNone: nothing).
 constexpr int kMaxOrder = 8 * kPairs;
 constexpr uint16_t kNone = 0xffff;
+constexpr int kAdd = 2;  // a tile's rows are added to what its item's earlier segments left
 struct Launch {
   Problem q[2];
   int items, positions, tabled;
@@ -139,6 +141,19 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                "r"(c0), "r"(c1), "r"(src)
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// The same with fp32 sums into what is there.
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's stores have reached global memory: its later ones to the same place come after them.
+__device__ __forceinline__ void tma_store_wait_done() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  fence_proxy_async_global();
 }
 // This thread's stores have read their shared memory.
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
@@ -244,14 +259,18 @@ __device__ __forceinline__ void add_row(uint32_t buf, int lane, float (&v)[Out<T
   for (int j = 0; j < 4; ++j) add16<T>(lds128(buf + chunk_at(lane, j)), v + j * (16 / sizeof(T)));
 }
 // A warp's 32 rows of a buffer in global memory, four lanes to a row: coalesced 16-byte accesses.
-template <typename T>
+// OWN: rows that this kernel has written (not to be had from the read-only cache).
+template <typename T, bool OWN = false>
 __device__ __forceinline__ void load_rows(const T* g, int64_t ld, int rows, int cols, int lane, uint4 (&v)[4]) {
   const int c = (lane & 3) * (16 / (int)sizeof(T));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = i * 8 + (lane >> 2);
     v[i] = make_uint4(0, 0, 0, 0);
-    if (r < rows && c < cols) v[i] = __ldg(reinterpret_cast<const uint4*>(g + r * ld + c));
+    if (r < rows && c < cols) {
+      const uint4* at = reinterpret_cast<const uint4*>(g + r * ld + c);
+      v[i] = OWN ? __ldcg(at) : __ldg(at);
+    }
   }
 }
 __device__ __forceinline__ void put_rows(uint32_t buf, int lane, const uint4 (&v)[4]) {
@@ -360,6 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_gemm_tc(const __grid_constant__ Launch l) {
   using L = Tile<BN>;
   constexpr int kCols = Out<T>::kCols;
+  constexpr bool kSegs = sizeof(T) == 4;  // an item may take several accumulators (fp32)
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   Bars* bars = reinterpret_cast<Bars*>(smem + L::OFF_BAR);
@@ -405,39 +425,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Problem& pr = l.q[TWO ? t.which : 0];
       const CUtensorMap *map_a = &pr.a, *map_b = &pr.b;
       const int a_mn = pr.p.a_mn, b_mn = pr.p.b_mn, fp32 = pr.p.fp32;
-      // fp32: a part of K goes through all plane pairs, `per` stages each
-      const int per = fp32 ? (t.i1 - t.i0) / kPlanePairs : 0, k0 = fp32 ? t.i0 / kPlanePairs : t.i0;
-      const int ma = t.m0 + (int)rank * 128, nb = t.n0 + (int)rank * (BN / 2);
-      const int skip = (mine + kLoaders - base % kLoaders) % kLoaders;
-      int s = (base + skip) % L::kStages;
-      uint32_t ph = ((base + skip) / L::kStages) & 1;  // the parity of the stage's round
-      int pair = fp32 ? skip / per : 0;
-      int kb = k0 + skip - pair * per;
-      for (int i = t.i0 + skip; i < t.i1; i += kLoaders) {
-        if (!(ok = wait(&bars->empty[s], ph ^ 1))) break;
-        if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
-        const uint32_t bar = full0 + s * 8;
-        const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
-        const int k = kb * kBK;
-        const int pa = fp32 ? plane_a(pair) : 0, pb = fp32 ? plane_b(pair) : 0;
-        if (a_mn) {
-          tma_load_pair(sa, map_a, ma, k, pa, bar);
-          tma_load_pair(sa + 8192, map_a, ma + 64, k, pa, bar);
-        } else {
-          tma_load_pair(sa, map_a, k, ma, pa, bar);
-        }
-        if (b_mn) {
+      const int ma = t.m0 + (int)rank * 128, nb = t.n0 + (int)rank * (BN / 2), seg = pr.p.seg;
+      for (int i0 = t.i0, i1; ok && i0 < t.i1; base += i1 - i0, i0 = i1) {
+        i1 = kSegs ? min(t.i1, i0 + seg) : t.i1;
+        // fp32: a segment of K goes through all plane pairs, `per` stages each
+        const int per = fp32 ? (i1 - i0) / kPlanePairs : 0, k0 = fp32 ? i0 / kPlanePairs : i0;
+        const int skip = (mine + kLoaders - base % kLoaders) % kLoaders;
+        int s = (base + skip) % L::kStages;
+        uint32_t ph = ((base + skip) / L::kStages) & 1;  // the parity of the stage's round
+        int pair = fp32 ? skip / per : 0;
+        int kb = k0 + skip - pair * per;
+        for (int i = i0 + skip; i < i1; i += kLoaders) {
+          if (!(ok = wait(&bars->empty[s], ph ^ 1))) break;
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * L::kStage);
+          const uint32_t bar = full0 + s * 8;
+          const uint32_t sa = sbase + s * L::kStage, sb = sa + kABytes;
+          const int k = kb * kBK;
+          const int pa = fp32 ? plane_a(pair) : 0, pb = fp32 ? plane_b(pair) : 0;
+          if (a_mn) {
+            tma_load_pair(sa, map_a, ma, k, pa, bar);
+            tma_load_pair(sa + 8192, map_a, ma + 64, k, pa, bar);
+          } else {
+            tma_load_pair(sa, map_a, k, ma, pa, bar);
+          }
+          if (b_mn) {
 #pragma unroll
-          for (int c = 0; c < BN / 128; ++c) tma_load_pair(sb + c * 8192, map_b, nb + c * 64, k, pb, bar);
-        } else {
-          tma_load_pair(sb, map_b, k, nb, pb, bar);
+            for (int c = 0; c < BN / 128; ++c) tma_load_pair(sb + c * 8192, map_b, nb + c * 64, k, pb, bar);
+          } else {
+            tma_load_pair(sb, map_b, k, nb, pb, bar);
+          }
+          kb += kLoaders;
+          while (fp32 && kb >= k0 + per) { kb -= per; ++pair; }
+          s += kLoaders;
+          if (s >= L::kStages) { s -= L::kStages; ph ^= 1; }
         }
-        kb += kLoaders;
-        while (fp32 && kb >= k0 + per) { kb -= per; ++pair; }
-        s += kLoaders;
-        if (s >= L::kStages) { s -= L::kStages; ph ^= 1; }
       }
-      base += t.i1 - t.i0;
     }
     // the last stages' loads and releases must have arrived before the CTAs may exit
     for (int j = max(0, base - L::kStages); mine == 0 && j < base; ++j) {
@@ -461,27 +483,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint64_t db = smem_desc(sbase + kABytes, p.b_mn ? 8192 : 16, 1024, kSwizzle128B);
       const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
       const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4, idesc = p.idesc;
-      const int buf = t & 1;
-      if (!(ok = wait(&bars->acc_free[buf], ((t >> 1) & 1) ^ 1))) break;
-      tc_fence_after();
-      const uint32_t d = tmem + buf * BN;
-      uint32_t more = 0;
-      for (int i = w.i0; i < w.i1; ++i) {
-        if (!(ok = wait(&bars->full[s], ph))) break;
+      const int seg = p.seg;
+      for (int i0 = w.i0, i1; ok && i0 < w.i1; i0 = i1, ++t) {
+        i1 = kSegs ? min(w.i1, i0 + seg) : w.i1;
+        const int buf = t & 1;
+        if (!(ok = wait(&bars->acc_free[buf], ((t >> 1) & 1) ^ 1))) break;
         tc_fence_after();
-        uint32_t a_lo = (uint32_t)da + s * (L::kStage >> 4), b_lo = (uint32_t)db + s * (L::kStage >> 4);
+        const uint32_t d = tmem + buf * BN;
+        uint32_t more = 0;
+        for (int i = i0; i < i1; ++i) {
+          if (!(ok = wait(&bars->full[s], ph))) break;
+          tc_fence_after();
+          uint32_t a_lo = (uint32_t)da + s * (L::kStage >> 4), b_lo = (uint32_t)db + s * (L::kStage >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 16; ++kk) {
-          mma_pair(d, ((uint64_t)a_hi << 32) | a_lo, ((uint64_t)b_hi << 32) | b_lo, idesc, more);
-          a_lo += a_step;
-          b_lo += b_step;
-          more = 1;
+          for (int kk = 0; kk < kBK / 16; ++kk) {
+            mma_pair(d, ((uint64_t)a_hi << 32) | a_lo, ((uint64_t)b_hi << 32) | b_lo, idesc, more);
+            a_lo += a_step;
+            b_lo += b_step;
+            more = 1;
+          }
+          commit_pair(&bars->empty[s]);
+          if (++s == L::kStages) { s = 0; ph ^= 1; }
         }
-        commit_pair(&bars->empty[s]);
-        if (++s == L::kStages) { s = 0; ph ^= 1; }
+        if (ok) commit_pair(&bars->acc_full[buf]);
       }
-      if (ok) commit_pair(&bars->acc_full[buf]);
-      ++t;
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
@@ -491,12 +516,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     pdl_wait();
     int t = 0;
     bool ok = true;
-    // sends the buffer's rows out, once every lane has written its own
+    // sends the buffer's rows out (tma = kAdd: adds them), once every lane has written its own
     auto send = [&](const CUtensorMap* map, int tma, T* base, int64_t ld, int row, int n, int store_row, int M, int N) {
       if (tma) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tma_store_2d(map, sbuf, n, store_row);
+        if (lane == 0) kSegs && tma == kAdd ? tma_add_2d(map, sbuf, n, store_row) : tma_store_2d(map, sbuf, n, store_row);
       } else {
         __syncwarp();
         copy_rows<T, true>(pbuf, base + (int64_t)row * ld + n, ld, min(32, M - row), N - n, lane);
@@ -512,69 +537,95 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Problem& pr = l.q[TWO ? it.which : 0];
       const Args& p = pr.p;
       const CUtensorMap* map_out = &pr.out;
-      const int M = p.M, N = p.N, out_tma = p.out_tma, partial = p.partial, split_row = it.split * p.split_rows;
-      const int buf = t & 1;
-      const int row = it.m0 + (int)rank * 128 + w * 32;
-      const int n_first = it.n0 + quarter * (BN / 4);
-      const int n_end = row < M ? min(N, n_first + BN / 4) : 0;
-      const T* res = TWO ? nullptr : static_cast<const T*>(p.res) + (int64_t)row * p.ldr;
-      const bool res_vec = !TWO && p.res && p.res_vec;
-      uint4 rv[4], bv[4];
-      if (res_vec && n_first < n_end)
-        load_rows(res + n_first, p.ldr, M - row, N - n_first, lane, rv);
-      if (!TWO && p.bias_vec && n_first < n_end) load_bias(static_cast<const T*>(p.bias) + n_first, N - n_first, bv);
-      ok = wait(&bars->acc_full[buf], (t >> 1) & 1);
-      ++t;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t acc = tmem + buf * BN + quarter * (BN / 4) + ((uint32_t)(w * 32) << 16);
-      for (int n = n_first; n < n_end; n += kCols) {
-        float v[kCols];
-        if constexpr (kCols == 32) tmem_ld32(acc + (n - n_first), v);
-        else tmem_ld16(acc + (n - n_first), v);
-        tmem_wait_ld();
-        if constexpr (sizeof(T) == 2) {
-          if (partial) {  // 32 columns of fp32: two rows' worth of the buffer
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              buffer_free();
-              write_row<float>(sbuf, lane, *reinterpret_cast<const float(*)[16]>(v + 16 * h));
-              send(map_out, 1, static_cast<T*>(nullptr), 0, row, n + 16 * h, split_row + row, M, N);
-            }
-            continue;
-          }
-        }
-        if (!TWO && p.bias) {
-          add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, bv, N - n, v);
-          if (p.bias_vec && n + kCols < n_end)
-            load_bias(static_cast<const T*>(p.bias) + n + kCols, N - n - kCols, bv);
-        }
-        if (!TWO && p.slope) {
-          buffer_free();
-          activate<T, true>(v, p.act, sbuf, lane);
-          send(&pr.slope, p.slope_tma, static_cast<T*>(p.slope), N, row, n, row, M, N);  // by size alone
-        } else if (!TWO) {
-          activate<T, false>(v, p.act, sbuf, lane);
-        }
-        buffer_free();
-        if (!TWO && p.res) {
-          if (res_vec) {
-            put_rows(sbuf, lane, rv);
-            if (n + kCols < n_end)
-              load_rows(res + n + kCols, p.ldr, M - row, N - n - kCols, lane, rv);
-          } else {
-            copy_rows<T, false>(pbuf, const_cast<T*>(res) + n, p.ldr, min(32, M - row), N - n, lane);
-          }
+      const int M = p.M, N = p.N, partial = p.partial, split_row = it.split * p.split_rows;
+      for (int i0 = it.i0; ok && i0 < it.i1; i0 = kSegs ? i0 + p.seg : it.i1) {
+        const bool later = kSegs && i0 > it.i0, last = !kSegs || i0 + p.seg >= it.i1;
+        const bool join = !TWO && later && last && p.join;
+        const int out_tma = later && !join ? kAdd : p.out_tma;
+        const int buf = t & 1;
+        const int row = it.m0 + (int)rank * 128 + w * 32;
+        const int n_first = it.n0 + quarter * (BN / 4);
+        const int n_end = row < M ? min(N, n_first + BN / 4) : 0;
+        const T* res = TWO ? nullptr : static_cast<const T*>(p.res) + (int64_t)row * p.ldr;
+        const bool res_vec = !TWO && p.res && p.res_vec;
+        uint4 rv[4], bv[4];
+        if (last && res_vec && n_first < n_end)
+          load_rows(res + n_first, p.ldr, M - row, N - n_first, lane, rv);
+        if (!TWO && last && p.bias_vec && n_first < n_end) load_bias(static_cast<const T*>(p.bias) + n_first, N - n_first, bv);
+        ok = wait(&bars->acc_full[buf], (t >> 1) & 1);
+        ++t;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (later) {
+          if (lane == 0) tma_store_wait_done();
           __syncwarp();
-          add_row<T>(sbuf, lane, v);
         }
-        write_row<T>(sbuf, lane, v);
-        send(map_out, out_tma, static_cast<T*>(p.out), p.ldo, row, n, split_row + row, M, N);
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * BN + quarter * (BN / 4) + ((uint32_t)(w * 32) << 16);
+        for (int n = n_first; n < n_end; n += kCols) {
+          float v[kCols];
+          if constexpr (kCols == 32) tmem_ld32(acc + (n - n_first), v);
+          else tmem_ld16(acc + (n - n_first), v);
+          tmem_wait_ld();
+          if constexpr (sizeof(T) == 2) {
+            if (partial) {  // 32 columns of fp32: two rows' worth of the buffer
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                buffer_free();
+                write_row<float>(sbuf, lane, *reinterpret_cast<const float(*)[16]>(v + 16 * h));
+                send(map_out, 1, static_cast<T*>(nullptr), 0, row, n + 16 * h, split_row + row, M, N);
+              }
+              continue;
+            }
+          }
+          if constexpr (kSegs && !TWO) {
+            if (!last) {
+              buffer_free();
+              write_row<T>(sbuf, lane, v);
+              send(map_out, out_tma, static_cast<T*>(nullptr), 0, row, n, split_row + row, M, N);
+              continue;
+            }
+            if (join) {
+              uint4 earlier[4];
+              load_rows<T, true>(static_cast<const T*>(p.out) + (int64_t)row * p.ldo + n, p.ldo, M - row, N - n, lane,
+                                 earlier);
+              buffer_free();
+              put_rows(sbuf, lane, earlier);
+              __syncwarp();
+              add_row<T>(sbuf, lane, v);
+            }
+          }
+          if (!TWO && p.bias) {
+            add_bias<T>(static_cast<const T*>(p.bias) + n, p.bias_vec, bv, N - n, v);
+            if (p.bias_vec && n + kCols < n_end)
+              load_bias(static_cast<const T*>(p.bias) + n + kCols, N - n - kCols, bv);
+          }
+          if (!TWO && p.slope) {
+            buffer_free();
+            activate<T, true>(v, p.act, sbuf, lane);
+            send(&pr.slope, p.slope_tma, static_cast<T*>(p.slope), N, row, n, row, M, N);  // by size alone
+          } else if (!TWO) {
+            activate<T, false>(v, p.act, sbuf, lane);
+          }
+          buffer_free();
+          if (!TWO && p.res) {
+            if (res_vec) {
+              put_rows(sbuf, lane, rv);
+              if (n + kCols < n_end)
+                load_rows(res + n + kCols, p.ldr, M - row, N - n - kCols, lane, rv);
+            } else {
+              copy_rows<T, false>(pbuf, const_cast<T*>(res) + n, p.ldr, min(32, M - row), N - n, lane);
+            }
+            __syncwarp();
+            add_row<T>(sbuf, lane, v);
+          }
+          write_row<T>(sbuf, lane, v);
+          send(map_out, out_tma, static_cast<T*>(p.out), p.ldo, row, n, split_row + row, M, N);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_remote(map_to_first(&bars->acc_free[buf]));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_remote(map_to_first(&bars->acc_free[buf]));
     }
     if (lane == 0) tma_store_wait_read();
   }
@@ -697,20 +748,46 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackArgs a
 // ---------------------------------------------------------------------------
 namespace {
 
-bool tma_rows(const void* p, int64_t ld, size_t es) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0;
-}
 int64_t pitch_of(int cols) { return ((int64_t)cols + 7) / 8 * 8; }
 
 struct Config {
   int bn, splits, iters, total, tiles_m, tiles_n;
+  int seg;       // stages per accumulator
+  bool partial;  // fp32 sums in the workspace, then k_split_sum
+  bool direct;   // fp32 sums in the result itself
 };
 
+bool tma_rows(const void* p, int64_t ld, size_t es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0;
+}
+bool bare(const Gemm& g) { return !g.bias && !g.res && !g.slope && g.act == MURM_ACT_NONE; }
+
+// The tensor cores cut each partial sum to 24 bits. So that fp32 keeps its accuracy whatever K is, an
+// accumulator of fp32 takes at most kSegment stages of K. An item's first segment is stored, each further
+// one added to it in global memory in fp32 (rounded; by the pair that stored it, in order; sums below
+// 2^-126 count as 0): in the result itself where K is not split and 16-byte rows allow it, and there the
+// last segment reads what the others left, if an epilogue follows. Error in parts of its norm and time, by
+// the most of K a segment takes (512, 768, 1024; all of it): 4096^3 5.2e-7 666 us, 7.0e-7 651, 1.05e-6 637,
+// 4.5e-6 613 (plain fp32 1.1e-6); 4096 x 1024 -> 4096 5.2e-7 165, the same, 1.05e-6 157 (5.7e-7); dW of 64 x 64
+// over 40000 rows 5.3e-7, 6.5e-7, 8.8e-7, all 86 us (8.4e-7).
+constexpr int kSegment = 768 / kBK;
+
 Config config(const Gemm& g, int bn, int splits) {
-  const int kblocks = (g.K + kBK - 1) / kBK, pairs = g.a.planes == 3 ? kPlanePairs : 1;
-  const int total = kblocks * pairs;
-  const int iters = (kblocks + splits - 1) / splits * pairs;
-  return Config{bn, (total + iters - 1) / iters, iters, total, (g.M + 255) / 256, (g.N + bn - 1) / bn};
+  const bool fp32 = g.a.planes == 3;
+  const int kblocks = (g.K + kBK - 1) / kBK, pairs = fp32 ? kPlanePairs : 1;
+  const int blocks = (kblocks + splits - 1) / splits;  // of a split
+  const int segments = fp32 ? (blocks + kSegment - 1) / kSegment : 1;
+  Config c{};
+  c.bn = bn;
+  c.total = kblocks * pairs;
+  c.iters = blocks * pairs;
+  c.splits = (c.total + c.iters - 1) / c.iters;
+  c.tiles_m = (g.M + 255) / 256;
+  c.tiles_n = (g.N + bn - 1) / bn;
+  c.seg = (blocks + segments - 1) / segments * pairs;
+  c.direct = c.splits == 1 && segments > 1 && tma_rows(g.out, g.ldo, 4) && g.N % 4 == 0 && g.res != g.out;
+  c.partial = !c.direct && (c.splits > 1 || segments > 1);
+  return c;
 }
 
 // Tile width and K splits by estimated time, in microseconds measured on B200:
@@ -724,26 +801,22 @@ Config config(const Gemm& g, int bn, int splits) {
 constexpr double kLaunchUs = 5.0;
 double stage_us(int bn) { return bn == 256 ? 0.35 : 0.31; }
 double split_us(const Config& c) {
-  return c.splits == 1 ? 0.0 : 4.0 + (double)c.tiles_m * c.tiles_n * 256 * c.bn * 4 * c.splits / 4.8e6;
+  const double tiles = (double)c.tiles_m * c.tiles_n * 256 * c.bn * 4 / 9.6e6;  // one pass over all
+  const double rest = c.partial ? 4.0 + tiles * c.splits : 0.0;  // k_split_sum
+  return c.partial || c.direct ? rest + tiles * ((c.total + c.seg - 1) / c.seg) : 0.0;
 }
-bool split_fits(const Config& c, int splits) {
-  return splits == 1 || (c.total / splits >= 2 && (int64_t)c.tiles_m * c.tiles_n * splits <= 2 * kPairs);
-}
-// The tensor cores cut each partial sum to 24 bits. So that fp32 keeps its accuracy, no accumulator
-// takes more than 1024 of K (16 parts at most, and as long as their sums fit 4 GB): 955 x 2064 -> 3224
-// has an error of 7.0e-7 of its norm in 97 us, 2.2e-6 in 79 with parts by time alone (a plain fp32
-// product 8.1e-7); 4096^3 1.1e-6 in 638 us, 4.5e-6 in 613 (1.2e-6).
-int least_splits(const Gemm& g) {
-  if (g.a.planes != 3) return 1;
-  const int parts = std::min((g.K + 1023) / 1024, 16);
-  return (int64_t)(g.M + 255) / 256 * ((g.N + 255) / 256) * parts <= (1 << 14) ? parts : 1;
+// fp32 items are six times as long, so that splits may pay for more of them (both gradients of 4200 x 1100
+// -> 4100: 470 us so, 550 with two rounds at most; of 4096^3 1180, with eight 1400).
+bool split_fits(const Gemm& g, const Config& c, int splits) {
+  const int most = (g.a.planes == 3 ? 4 : 2) * kPairs;
+  return splits == 1 || (c.total / splits >= 2 && (int64_t)c.tiles_m * c.tiles_n * splits <= most);
 }
 double choose_one(const Gemm& g, Config* best) {
   double best_t = 0;
   for (int bn : {256, 128})
-    for (int splits = least_splits(g), least = splits; splits <= 16; ++splits) {
+    for (int splits = 1; splits <= 16; ++splits) {
       const Config c = config(g, bn, splits);
-      if (splits > least && !split_fits(c, splits)) break;
+      if (!split_fits(g, c, splits)) break;
       const int64_t rounds = ((int64_t)c.tiles_m * c.tiles_n * c.splits + kPairs - 1) / kPairs;
       const double t = rounds * c.iters * stage_us(bn) + split_us(c);
       if (best_t == 0 || t < best_t) {
@@ -780,8 +853,7 @@ Plan choose(const Gemm* g, int count) {
       for (int splits : kSplits) {
         Option& o = opt[i][n[i]];
         o.c = config(g[i], bn, splits);
-        if (splits < least_splits(g[i])) continue;
-        if (n[i] && !split_fits(o.c, splits)) break;
+        if (!split_fits(g[i], o.c, splits)) break;
         o.item = o.c.iters * stage_us(bn);
         o.work = o.item * o.c.tiles_m * o.c.tiles_n * o.c.splits;
         o.extra = split_us(o.c);
@@ -868,7 +940,7 @@ CUresult describe(const Gemm& g, const Config& c, void* workspace, Problem* q) {
   Args& p = q->p;
   p = Args{};
   p.M = g.M; p.N = g.N;
-  p.iters = c.iters; p.total = c.total; p.splits = c.splits;
+  p.iters = c.iters; p.total = c.total; p.splits = c.splits; p.seg = c.seg;
   p.tiles_m = c.tiles_m;
   p.tiles_n = c.tiles_n;
   p.tiles = c.tiles_m * c.tiles_n;
@@ -885,7 +957,7 @@ CUresult describe(const Gemm& g, const Config& c, void* workspace, Problem* q) {
   if (g.b_mn) r = encode(&q->b, op, 2, g.b.p, g.N, g.K, g.b.ld, g.b.planes, g.b.plane, 64, 64);
   else r = encode(&q->b, op, 2, g.b.p, g.K, g.N, g.b.ld, g.b.planes, g.b.plane, 64, BN / 2);
   if (r != CUDA_SUCCESS) return r;
-  if (c.splits > 1) {  // partial sums alone; the epilogue follows in k_split_sum
+  if (c.partial) {  // partial sums alone; the epilogue follows in k_split_sum
     p.partial = 1;
     p.M = p.split_rows = c.tiles_m * 256;
     p.N = c.tiles_n * BN;
@@ -899,6 +971,7 @@ CUresult describe(const Gemm& g, const Config& c, void* workspace, Problem* q) {
   p.res = g.res; p.ldr = g.ldr;
   p.out = g.out; p.ldo = g.ldo;
   p.slope = g.slope;
+  p.join = c.direct && !bare(g);
   const int per = 16 / (int)es;
   p.res_vec = p.res && tma_rows(p.res, p.ldr, es) && g.N % per == 0;
   p.bias_vec = p.bias && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && g.N % per == 0;
@@ -912,7 +985,7 @@ CUresult describe(const Gemm& g, const Config& c, void* workspace, Problem* q) {
 }
 
 size_t split_bytes(const Config& c) {
-  return c.splits == 1 ? 0 : (size_t)c.splits * c.tiles_m * 256 * c.tiles_n * c.bn * sizeof(float);
+  return !c.partial ? 0 : (size_t)c.splits * c.tiles_m * 256 * c.tiles_n * c.bn * sizeof(float);
 }
 
 // One launch of one or two products with the same tile width, then the sums of those with splits.
@@ -942,7 +1015,7 @@ murm_status launch_tc(const Gemm* g, const Config* c, int count, char* workspace
   if (cudaError_t e = smem_opt_in(kernel, Tile<BN>::kSmem)) return report_error(MURM_ERR_CUDA, cudaGetErrorString(e));
   launch("linear_gemm", kernel, dim3(2 * pairs), kThreads, Tile<BN>::kSmem, st, l);
   for (int i = 0; i < count; ++i) {
-    if (c[i].splits == 1) continue;
+    if (!c[i].partial) continue;
     Args p = l.q[i ^ swap].p;
     const int ldp = p.N;
     const int64_t stride = (int64_t)p.M * p.N;
