@@ -425,9 +425,11 @@ MURM_API size_t murm_norm_rope_workspace(void);
  * residual and out [rows, out_features] likewise, bias [out_features]. Sums
  * are in fp32 (fp32 inputs: exact three-term bf16 splits, fp32 accuracy).
  * slope, when not NULL, receives act'(z) ([rows, out_features] contiguous; fp32
- * beside fp32, beside 16-bit tensors uint16 codes c of (c - 8192) / 32768 with
- * 65535 for NaN) for the backward; it is needed there unless the activation is
- * MURM_ACT_NONE, which writes none.
+ * beside fp32, beside 16-bit tensors uint16 codes) for the backward; it is needed
+ * there unless the activation is MURM_ACT_NONE, which writes none. A code c below
+ * 0xc000 is (c - 8192) / 32768, within 2^-16; from 0xc000 on it is a small slope
+ * rounded to `dtype` (below 2^-7 for fp16, 2^-8 for bf16), with the sign in bit 13 and
+ * below it the number's last 13 bits (bf16: of the slope times 2^-55); 65535 is NaN.
  *
  * Backward: dz = grad_out * slope, rounded once to `dtype` where it becomes a
  * matrix operand; grad_x = dz W, grad_weight = dz^T x, grad_bias = column sums of

@@ -203,8 +203,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t pack2(float a, float b, const SlopeCode*) {
-  return __byte_perm(slope_bits(a), slope_bits(b), 0x5410);
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b, const SlopeCode<T>*) {
+  return encode_slopes<T>(a, b);
 }
 __device__ __forceinline__ float2 unpack2(uint32_t u, const __half*) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
@@ -326,7 +327,10 @@ __device__ __forceinline__ void activate_as(float (&v)[Out<T>::kCols], uint32_t 
     float d[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[j * kPer + i] = act_value<Out<T>::kFast>(v[j * kPer + i], ACT, d[i]);
-    if (SLOPE) sts128(buf + chunk_at(lane, j), pack16<Slope<T>>(d));
+    if constexpr (SLOPE && ACT == MURM_ACT_RELU && sizeof(T) == 2)  // 0 and 1 are steps
+      sts128(buf + chunk_at(lane, j), make_uint4(slope_steps(d[0], d[1]), slope_steps(d[2], d[3]),
+                                                 slope_steps(d[4], d[5]), slope_steps(d[6], d[7])));
+    else if (SLOPE) sts128(buf + chunk_at(lane, j), pack16<Slope<T>>(d));
   }
 }
 template <typename T, bool SLOPE>

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kDzThreads, 3)
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
   auto row = [&](int r, const P& g, const PS& sl) {
     float d[V], s[V];
-    if (SLOPE) load_slopes<V>(sl.e, s);
+    if (SLOPE) load_slopes(sl.e, s);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       d[e] = Elem<T>::load(g.e + e);

@@ -33,48 +33,106 @@ struct Gemm {
 size_t gemm_workspace(const Gemm* g, int count);
 murm_status gemm(const Gemm* g, int count, void* workspace, cudaStream_t st);
 
-// A slope in 16 bits: (code - 8192) 2^-15, so -0.25 to 1.75 in equal steps with 0 and 1 exact (the
-// activations' slopes lie between -0.13 and 1.13), within 2^-16; code 65535 is NaN. Both ways are one
-// fma: added to 2^23, the number's last mantissa bits are the code (a NaN's are all ones).
-struct SlopeCode { uint16_t code; };
+// A slope beside elements of 16 bits T, in 16 bits. The activations' slopes lie between -0.13 and 1.13.
+// - codes below 0xc000: (code - 8192) 2^-15, equal steps with 1 exact, within 2^-16; both ways are one
+//   fma: added to 2^23, the number's last mantissa bits are the code.
+// - from 0xc000 on: small slopes, as the T they round to. Bit 13 is the sign, the bits below it T's last 13:
+//   fp16 below 2^-7, and bf16 below 2^-8 (held times 2^-55, so that 13 bits reach to 2^-71). In equal steps a
+//   unit in its activation's tail would get a wrong gradient or none (gelu's slope 11 % off at -4.5, zero
+//   from -5 on) where T can hold the right one.
+// - 0xffff: NaN (a NaN's last bits are ones after the fma; the largest small slope is left out for it).
+// fp16 slopes throughout, within 2^-12 of those near one, gave fp16 gradients 1.2 times the error.
+template <typename T> struct SlopeCode { uint16_t code; };
 constexpr float kSlopeScale = 32768.f, kSlopeZero = 8388608.f + 8192.f;
 __device__ __forceinline__ uint32_t slope_bits(float s) { return __float_as_uint(fmaf(s, kSlopeScale, kSlopeZero)); }
-
-// Type of the saved slopes: fp32 beside fp32, else codes. (fp16 slopes, within 2^-12 of those near one,
-// gave fp16 gradients 1.2 times the error: 3.4e-4 of their norm.)
-template <typename T> struct SlopeOf { using type = SlopeCode; };
-template <> struct SlopeOf<float> { using type = float; };
-template <typename T> using Slope = typename SlopeOf<T>::type;
-__device__ __forceinline__ void store_slope(float* p, float s) { *p = s; }
-__device__ __forceinline__ void store_slope(SlopeCode* p, float s) { p->code = (uint16_t)slope_bits(s); }
 __device__ __forceinline__ float slope_of(uint32_t bits) {  // 0x4b000000 | code
   return fmaf(__uint_as_float(bits), 1.f / kSlopeScale, -kSlopeZero / kSlopeScale);
 }
+constexpr float kSmallCodes = 1.25f;          // what the fma makes of 0xc000
+constexpr uint32_t kSmallEnd = 0x1fff1fffu;   // in T's bits, twice
+constexpr float kBf16Down = 0x1p-55f, kBf16Up = 0x1p55f;
+// Two slopes as the T's of small ones, and 0xffff where they are small enough.
+__device__ __forceinline__ uint32_t small_slopes(float a, float b, uint32_t& mask, const __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  uint32_t bits, end = kSmallEnd;
+  __half2 limit;
+  memcpy(&limit, &end, 4);
+  mask = __hlt2_mask(__habs2(h), limit);
+  memcpy(&bits, &h, 4);
+  return bits;
+}
+__device__ __forceinline__ uint32_t small_slopes(float a, float b, uint32_t& mask, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a * kBf16Down, b * kBf16Down);
+  uint32_t bits, end = kSmallEnd;
+  __nv_bfloat162 limit;
+  memcpy(&limit, &end, 4);
+  mask = __hlt2_mask(__habs2(h), limit);
+  memcpy(&bits, &h, 4);
+  return bits;
+}
+__device__ __forceinline__ void small_values(uint32_t bits, float& a, float& b, const __half*) {
+  __half2 h;
+  memcpy(&h, &bits, 4);
+  const float2 f = __half22float2(h);
+  a = f.x;
+  b = f.y;
+}
+__device__ __forceinline__ void small_values(uint32_t bits, float& a, float& b, const __nv_bfloat16*) {
+  a = __uint_as_float(bits << 16) * kBf16Up;
+  b = __uint_as_float(bits & 0xffff0000u) * kBf16Up;
+}
+// Two slopes <-> two codes, the first in the low half.
+__device__ __forceinline__ uint32_t slope_steps(float a, float b) {
+  return __byte_perm(slope_bits(a), slope_bits(b), 0x5410);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t encode_slopes(float a, float b) {
+  const uint32_t steps = slope_steps(a, b);
+  uint32_t mask;
+  const uint32_t bits = small_slopes(a, b, mask, (const T*)nullptr);
+  return ((bits | ((bits >> 2) & 0x20002000u) | 0xc000c000u) & mask) | (steps & ~mask);
+}
+template <typename T>
+__device__ __forceinline__ void decode_slopes(uint32_t w, float& a, float& b) {  // all but NaN
+  float sa, sb;
+  small_values((w & 0x1fff1fffu) | ((w << 2) & 0x80008000u), sa, sb, (const T*)nullptr);
+  a = slope_of(__byte_perm(w, 0x4b00u, 0x5410));
+  b = slope_of(__byte_perm(w, 0x4b00u, 0x5432));
+  a = a >= kSmallCodes ? sa : a;
+  b = b >= kSmallCodes ? sb : b;
+}
+
+// Type of the saved slopes: fp32 beside fp32, else codes.
+template <typename T> struct SlopeOf { using type = SlopeCode<T>; };
+template <> struct SlopeOf<float> { using type = float; };
+template <typename T> using Slope = typename SlopeOf<T>::type;
+__device__ __forceinline__ void store_slope(float* p, float s) { *p = s; }
+template <typename T>
+__device__ __forceinline__ void store_slope(SlopeCode<T>* p, float s) { p->code = (uint16_t)encode_slopes<T>(s, s); }
 template <int V>
 __device__ __forceinline__ void load_slopes(const float (&s)[V], float (&out)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) out[e] = s[e];
 }
-// Two codes to a word. No slope's code has both upper bits set, so one test over all the words tells
-// whether one is NaN (a comparison per code made 4096 x 1024 a microsecond slower).
-template <int V>
-__device__ __forceinline__ void load_slopes(const SlopeCode (&s)[V], float (&out)[V]) {
-  uint32_t nan = 0;
+// Two codes to a word. One maximum over all the words tells whether one of them is NaN (a comparison per code
+// made 4096 x 1024 a microsecond slower).
+template <typename T, int V>
+__device__ __forceinline__ void load_slopes(const SlopeCode<T> (&s)[V], float (&out)[V]) {
+  uint32_t most = 0;
   if constexpr (V == 1) {
-    nan = s[0].code;
-    out[0] = slope_of(0x4b000000u | nan);
-    nan &= nan << 1;
+    float unused;
+    most = s[0].code;
+    decode_slopes<T>(most, out[0], unused);
   } else {
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
       uint32_t w;
       memcpy(&w, &s[e], sizeof(w));
-      nan |= w & (w << 1);
-      out[e] = slope_of(__byte_perm(w, 0x4b00u, 0x5410));
-      out[e + 1] = slope_of(__byte_perm(w, 0x4b00u, 0x5432));
+      most = __vmaxu2(most, w);
+      decode_slopes<T>(w, out[e], out[e + 1]);
     }
   }
-  if (nan & 0x80008000u) {
+  if ((most & 0xffffu) == 0xffffu || most >= 0xffff0000u) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
       if (s[e].code == 0xffffu) out[e] = __uint_as_float(0x7fffffffu);
