@@ -155,31 +155,48 @@ __global__ void __launch_bounds__(1024) k_col_sum(const float* part, int chunks,
   if (lane == 0 && blockIdx.x * 32 + warp < N) Elem<T>::store(out + blockIdx.x * 32 + warp, sum);
 }
 
-template <typename T, int V>
-void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cudaStream_t st) {
-  const int M = (int)a.rows, N = a.out_features;
-  int cols = 32;
-  while (cols < kDzThreads && cols * V < N) cols *= 2;
-  const int blocks_x = (N + cols * V - 1) / (cols * V);
+// The pass's blocks: `cols` threads side by side with V columns each, chunks of `chunk` rows.
+struct DzShape {
+  int v, cols, blocks_x, chunk, chunks;
+};
+DzShape dz_shape(const murm_linear_bwd_args& a) {
+  const int M = (int)a.rows, N = a.out_features, v = 16 / (a.dtype == MURM_F32 ? 4 : 2);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.grad_out) | reinterpret_cast<uintptr_t>(a.slope);
+  DzShape s{};
+  s.v = N % v == 0 && a.go_stride % v == 0 && bits % 16 == 0 ? v : 1;
+  s.cols = 32;
+  while (s.cols < kDzThreads && s.cols * s.v < N) s.cols *= 2;
+  s.blocks_x = (int)(((int64_t)N + s.cols * s.v - 1) / (s.cols * s.v));
   // Two rounds of three blocks per SM, so that the last ones leave little idle. With slopes one round
   // where two would leave a thread less than 64 rows, and 24 rows per chunk at least (bf16 8192 x 4096,
   // gradients of 64 inputs with it: one round of 37 rows 70 us, 32 rows in 1.15 rounds 78; 4096 x 1024:
   // chunks of 24 rows 18.2, of 32 19.1, of 48 20.6). Without them, half the bytes, 32 rows and two rounds
   // (8192 x 4096: 42.0, one round 43.5).
   const bool slopes = a.activation != MURM_ACT_NONE;
-  const int wave = 148 * 3 / blocks_x, least = slopes ? 24 : 32;
+  const int wave = 148 * 3 / s.blocks_x, least = slopes ? 24 : 32;
   int most = 2 * wave;
-  if (slopes && (int64_t)most * 64 * (kDzThreads / cols) > M) most = wave;
+  if (slopes && (int64_t)most * 64 * (kDzThreads / s.cols) > M) most = wave;
   if (most < 1) most = 1;
   if (most > kDzChunks) most = kDzChunks;
   if (most > (M + least - 1) / least) most = (M + least - 1) / least;
   // few rows per thread in all: one chunk, whose block writes db itself (a launch less)
-  if (M <= 16 * (kDzThreads / cols)) most = 1;
-  const int chunk = (M + most - 1) / most;
-  const int chunks = (M + chunk - 1) / chunk;
-  const dim3 grid(blocks_x, chunks);
+  if (M <= 16 * (kDzThreads / s.cols)) most = 1;
+  s.chunk = (M + most - 1) / most;
+  s.chunks = (M + s.chunk - 1) / s.chunk;
+  return s;
+}
+// Partial sums of db: one chunk writes db itself.
+size_t dz_part_bytes(const murm_linear_bwd_args& a) {
+  const int chunks = a.grad_bias ? dz_shape(a).chunks : 0;
+  return chunks > 1 ? (size_t)chunks * a.out_features * sizeof(float) : 0;
+}
+
+template <typename T, int V>
+void launch_dz(const murm_linear_bwd_args& a, const DzShape& s, const Operand& dz, float* part, cudaStream_t st) {
+  const int M = (int)a.rows, N = a.out_features, cols = s.cols, chunk = s.chunk, chunks = s.chunks;
+  const dim3 grid(s.blocks_x, chunks);
   const T* dy = static_cast<const T*>(a.grad_out);
-  T* db = part && chunks == 1 ? static_cast<T*>(a.grad_bias) : nullptr;
+  T* db = chunks == 1 ? static_cast<T*>(a.grad_bias) : nullptr;
   if (db) part = nullptr;
   if (a.activation == MURM_ACT_NONE)
     MURM_LAUNCH_PDL("linear_col_part", (k_dz<T, V, false>), grid, kDzThreads, 0, st, dy, a.go_stride,
@@ -195,11 +212,9 @@ void launch_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cu
 template <typename T>
 void run_dz(const murm_linear_bwd_args& a, const Operand& dz, float* part, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.grad_out) | reinterpret_cast<uintptr_t>(a.slope);
-  if (a.out_features % V == 0 && a.go_stride % V == 0 && bits % 16 == 0)
-    launch_dz<T, V>(a, dz, part, st);
-  else
-    launch_dz<T, 1>(a, dz, part, st);
+  const DzShape s = dz_shape(a);
+  if (s.v == V) launch_dz<T, V>(a, s, dz, part, st);
+  else launch_dz<T, 1>(a, s, dz, part, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -356,7 +371,7 @@ BwdPlan plan_bwd(const murm_linear_bwd_args& a) {
   }
   if (a.grad_x) p.w = p.l.source(a.weight, a.w_stride, a.out_features, a.in_features);
   if (a.grad_weight) p.x = p.l.source(a.x, a.x_stride, a.rows, a.in_features);
-  p.part_at = p.l.take(a.grad_bias ? (size_t)kDzChunks * a.out_features * sizeof(float) : 0);
+  p.part_at = p.l.take(dz_part_bytes(a));
   Gemm g{};
   g.dtype = a.dtype;
   g.a = p.dz;

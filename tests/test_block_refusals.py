@@ -118,3 +118,15 @@ def test_sizes_past_32_bits_are_refused(fake, big):
             binding.rotary(fake(*shape), p, *rest, False)
         with pytest.raises(RuntimeError, match="2\\^31"):
             binding.qk_norm_rope(fake(*shape), None, p, None, None, 1e-6, *rest)
+
+
+@pytest.mark.parametrize("rows,n", [(8, 1 << 24), (300, 1 << 20), (8, (1 << 31) - 1032), (20000, 64), (5000, 100000)])
+@pytest.mark.parametrize("act", [0, 1])
+def test_bias_gradient_needs_no_more_than_its_chunks(rows, n, act):
+    """The partial sums of db alone: at most one row of them per 24 rows of dz, none where one block sums a
+    column (512 rows of them whatever the sizes took 34 GB beside 2^24 outputs)."""
+    a = _lib.LinearBwdArgs(rows=rows, in_features=64, out_features=n, dtype=_lib.MURM_BF16, activation=act, slope=4096,
+                           grad_out=8192, go_stride=n, grad_bias=16384)
+    need = ctypes.c_size_t(0)
+    assert _lib.load_library().murm_linear_bwd_workspace(ctypes.byref(a), ctypes.byref(need)) == 0
+    assert need.value <= (rows // 24 + 1) * n * 4 * (rows > 16) + 256
