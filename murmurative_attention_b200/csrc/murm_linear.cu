@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kDzThreads, 3)
   sm100::pdl_wait();
   sm100::pdl_trigger();
   const int tx = threadIdx.x & (cols - 1), ty = threadIdx.x / cols, rows = kDzThreads / cols;
-  const int n = (blockIdx.x * cols + tx) * V;
+  const uint32_t n = (blockIdx.x * cols + tx) * (uint32_t)V;  // the last block's may pass 2^31
   const int m1 = (int)min((int64_t)M, (int64_t)(blockIdx.y + 1) * chunk);
   constexpr int kDepth = SLOPE ? kDzDepth : 2 * kDzDepth;
   using P = Pack<T, V>;
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kDzThreads, 3)
     }
     if (SLOPE && dz.p) store_operand<T, V>(dz, (int64_t)r * dz.ld + n, d);
   };
-  if (n < N) {  // V divides N
+  if (n < (uint32_t)N) {  // V divides N
     int m = blockIdx.y * chunk + ty;
     const T* pg = dy + (int64_t)m * ldy + n;
     const Slope<T>* ps = slope + (int64_t)m * N + n;
@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(kDzThreads, 3)
   for (int e = 0; e < V; ++e) s[(ty * cols + tx) * V + e] = acc[e];
   __syncthreads();
   for (int c = threadIdx.x; c < cols * V; c += kDzThreads) {
-    const int col = blockIdx.x * cols * V + c;
-    if (col >= N) continue;
+    const uint32_t col = blockIdx.x * cols * (uint32_t)V + c;
+    if (col >= (uint32_t)N) continue;
     float sum = 0.f;
     for (int r = 0; r < rows; ++r) sum += s[r * cols * V + c];
     if (db) Elem<T>::store(db + col, sum);  // the only chunk

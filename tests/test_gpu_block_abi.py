@@ -76,3 +76,19 @@ def test_nothing_rotated_needs_no_positions(dtype):
     set_rows(a.q, x, copy)
     run(a)
     assert torch.equal(copy, x)
+
+
+def test_bias_gradient_of_the_widest_layer():
+    """Column offsets pass 2^31 in the last block; one row, so that the sums are its elements."""
+    n = (1 << 31) - 1032
+    go = torch.empty(n, dtype=torch.bfloat16, device="cuda")
+    go.view(torch.int16).copy_(torch.arange(1 << 14, device="cuda", dtype=torch.int16).repeat((n >> 14) + 1)[:n])
+    gb = torch.full_like(go, NAN)
+    a = _lib.LinearBwdArgs(rows=1, in_features=1, out_features=n, dtype=_lib.MURM_BF16, grad_out=go.data_ptr(), go_stride=n,
+                           grad_bias=gb.data_ptr())
+    need = ctypes.c_size_t(0)
+    lib = _lib.load_library()
+    assert lib.murm_linear_bwd_workspace(ctypes.byref(a), ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.murm_linear_bwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(gb, go)
