@@ -299,7 +299,8 @@ Tensor fused_linear(const Tensor& x, const Tensor& weight, const optional<Tensor
       (wants_grad(x2) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))) {
     auto node = make_node<FusedLinearBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(x2, weight, bias, residual));
-    std::tie(out, slope) = linear_forward(x2, weight, bias, residual, act, true);
+    const bool save = wants_grad(x2) || wants_grad(weight) || wants_grad(bias);  // the residual's gradient needs none
+    std::tie(out, slope) = linear_forward(x2, weight, bias, residual, act, save);
     node->act = act;
     node->x = SavedVariable(x2, false);
     node->weight = SavedVariable(weight, false);
@@ -617,7 +618,7 @@ Tensor or_empty(const Tensor& t, const Tensor& like) { return t.defined() ? t : 
 void check_rows_2d(const Tensor& x) { TORCH_CHECK(x.dim() == 2, "x must be [M, K], got ", x.sizes()); }
 
 std::tuple<Tensor, Tensor> linear_fwd(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias,
-                                      const std::string& activation, const optional<Tensor>& residual_) {
+                                      const std::string& activation, const optional<Tensor>& residual_, bool save) {
   const int64_t act = activation_code(activation);
   const Tensor residual = value(residual_);
   check_linear(x, weight, value(bias), residual);
@@ -625,11 +626,12 @@ std::tuple<Tensor, Tensor> linear_fwd(const Tensor& x, const Tensor& weight, con
   TORCH_CHECK(!residual.defined() || (residual.dim() == 2 && residual.size(0) == x.size(0) &&
                                       residual.size(1) == weight.size(0)),
               "residual must be [M=", x.size(0), ", N=", weight.size(0), "], got ", residual.sizes());
-  auto [out, slope] = linear_forward(x, weight, value(bias), residual, act, true);
+  auto [out, slope] = linear_forward(x, weight, value(bias), residual, act, save);
   return {out, or_empty(slope, x)};
 }
 std::tuple<Tensor, Tensor, Tensor> linear_bwd(const Tensor& go, const Tensor& x, const Tensor& weight,
-                                              const Tensor& slope, const std::string& activation) {
+                                              const Tensor& slope, const std::string& activation, bool need_x,
+                                              bool need_weight, bool need_bias) {
   const int64_t act = activation_code(activation);
   check_linear(x, weight, Tensor(), go);
   check_rows_2d(x);
@@ -644,7 +646,9 @@ std::tuple<Tensor, Tensor, Tensor> linear_bwd(const Tensor& go, const Tensor& x,
     TORCH_CHECK(slope.sizes() == shape && slope.is_contiguous(), "slope must be contiguous and ", shape, ", got ",
                 slope.sizes());
   }
-  return linear_backward(go, x, weight, act != MURM_ACT_NONE ? slope : Tensor(), act, true, true, true);
+  const auto [gx, gw, gb] =
+      linear_backward(go, x, weight, act != MURM_ACT_NONE ? slope : Tensor(), act, need_x, need_weight, need_bias);
+  return {or_empty(gx, x), or_empty(gw, x), or_empty(gb, x)};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> qk_bwd(const Tensor& gq, const Tensor& gk, const Tensor& q,
                                                   const optional<Tensor>& k_, const Tensor& positions,
@@ -677,7 +681,9 @@ PYBIND11_MODULE(_murm_torch, m) {
   m.def("fused_linear", &fused_linear);
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("rotary", &rotary);
-  m.def("linear_fwd", &linear_fwd);
-  m.def("linear_bwd", &linear_bwd);
+  m.def("linear_fwd", &linear_fwd, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("activation"),
+        py::arg("residual"), py::arg("save") = true);
+  m.def("linear_bwd", &linear_bwd, py::arg("grad_out"), py::arg("x"), py::arg("weight"), py::arg("slope"),
+        py::arg("activation"), py::arg("need_x") = true, py::arg("need_weight") = true, py::arg("need_bias") = true);
   m.def("qk_bwd", &qk_bwd);
 }

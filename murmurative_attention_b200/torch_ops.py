@@ -70,10 +70,10 @@ NORTH_STAR_SCHEMAS = {
 _ROTATION = ("float eps, float base, int? rotary_dim, bool interleaved, int[]? sections, str spectrum, "
              "Tensor? freqs")
 BLOCK_SCHEMAS = {
-    "fused_linear_fwd": "fused_linear_fwd(Tensor x, Tensor weight, Tensor? bias, str activation, Tensor? residual) "
-                        "-> (Tensor, Tensor)",
-    "fused_linear_bwd": "fused_linear_bwd(Tensor grad_out, Tensor x, Tensor weight, Tensor slope, str activation) "
-                        "-> (Tensor, Tensor, Tensor)",
+    "fused_linear_fwd": "fused_linear_fwd(Tensor x, Tensor weight, Tensor? bias, str activation, Tensor? residual, "
+                        "bool save=True) -> (Tensor, Tensor)",
+    "fused_linear_bwd": "fused_linear_bwd(Tensor grad_out, Tensor x, Tensor weight, Tensor slope, str activation, "
+                        "bool need_x=True, bool need_weight=True, bool need_bias=True) -> (Tensor, Tensor, Tensor)",
     "qk_norm_rope": f"qk_norm_rope(Tensor q, Tensor? k, Tensor positions, Tensor? q_weight, Tensor? k_weight, "
                     f"{_ROTATION}) -> (Tensor, Tensor)",
     "qk_norm_rope_bwd": f"qk_norm_rope_bwd(Tensor grad_q, Tensor grad_k, Tensor q, Tensor? k, Tensor positions, "
@@ -270,8 +270,8 @@ def slot_murmurate(q: Tensor, slots_k: Tensor, slots_v: Tensor, rounds: int = 3,
 # The block's operators (compiled binding over the C ABI)
 # ---------------------------------------------------------------------------
 @torch.library.impl(_q("fused_linear_fwd"), "CUDA", lib=_LIB)
-def _linear_fwd_cuda(x, weight, bias, activation, residual):
-    return _native.binding().linear_fwd(x, weight, bias, activation, residual)
+def _linear_fwd_cuda(x, weight, bias, activation, residual, save=True):
+    return _native.binding().linear_fwd(x, weight, bias, activation, residual, save)
 
 
 _LINEAR_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -310,24 +310,24 @@ def _check_outputs(t: Tensor, x: Tensor, weight: Tensor, name: str) -> None:
 
 
 @torch.library.register_fake(_q("fused_linear_fwd"), lib=_LIB)
-def _linear_fwd_fake(x, weight, bias, activation, residual):
+def _linear_fwd_fake(x, weight, bias, activation, residual, save=True):
     _check_linear(x, weight, activation, bias)
     if residual is not None:
         _like(residual, x, "residual")
         _check_outputs(residual, x, weight, "residual")
     out = x.new_empty(x.shape[0], weight.shape[0])
-    if activation == "none":
+    if activation == "none" or not save:
         return out, x.new_empty(0)
     return out, torch.empty_like(out, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
 
 
 @torch.library.impl(_q("fused_linear_bwd"), "CUDA", lib=_LIB)
-def _linear_bwd_cuda(grad_out, x, weight, slope, activation):
-    return _native.binding().linear_bwd(grad_out, x, weight, slope, activation)
+def _linear_bwd_cuda(grad_out, x, weight, slope, activation, need_x=True, need_weight=True, need_bias=True):
+    return _native.binding().linear_bwd(grad_out, x, weight, slope, activation, need_x, need_weight, need_bias)
 
 
 @torch.library.register_fake(_q("fused_linear_bwd"), lib=_LIB)
-def _linear_bwd_fake(grad_out, x, weight, slope, activation):
+def _linear_bwd_fake(grad_out, x, weight, slope, activation, need_x=True, need_weight=True, need_bias=True):
     _check_linear(x, weight, activation)
     _like(grad_out, x, "grad_out")
     _check_outputs(grad_out, x, weight, "grad_out")
@@ -336,20 +336,24 @@ def _linear_bwd_fake(grad_out, x, weight, slope, activation):
         _refuse(slope.dtype != kind, f"slope must be {kind} beside {x.dtype}, got {slope.dtype}", TypeError)
         _refuse(slope.device != x.device, f"slope must be on {x.device}, got {slope.device}")
         _check_outputs(slope, x, weight, "slope")
-    return x.new_empty(x.shape), x.new_empty(weight.shape), x.new_empty(weight.shape[0])
+    return tuple(x.new_empty(shape if need else 0) for shape, need in
+                 ((x.shape, need_x), (weight.shape, need_weight), (weight.shape[0], need_bias)))
 
 
 def _linear_setup(ctx, inputs, output):
-    x, weight, bias, activation, residual = inputs
+    x, weight, bias, activation, residual, _ = inputs
     ctx.save_for_backward(x, weight, output[1])
-    ctx.activation, ctx.has = activation, (bias is not None, residual is not None)
+    ctx.activation = activation
     ctx.mark_non_differentiable(output[1])
 
 
 def _linear_backward(ctx, grad_out, grad_slope):
     x, weight, slope = ctx.saved_tensors
-    gx, gw, gb = torch.ops.murmurative_attention.fused_linear_bwd(grad_out, x, weight, slope, ctx.activation)
-    return gx, gw, gb if ctx.has[0] else None, None, grad_out if ctx.has[1] else None
+    need = ctx.needs_input_grad
+    grads = [None, None, None]
+    if any(need[:3]):
+        grads = torch.ops.murmurative_attention.fused_linear_bwd(grad_out, x, weight, slope, ctx.activation, *need[:3])
+    return tuple(g if n else None for g, n in zip(grads, need)) + (None, grad_out if need[4] else None, None)
 
 
 torch.library.register_autograd(_q("fused_linear_fwd"), _linear_backward, setup_context=_linear_setup, lib=_LIB)
@@ -363,7 +367,8 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: 
     shape = x.shape[:-1] + (weight.shape[0],)
     x2 = x.reshape(-1, x.shape[-1])
     r2 = residual.expand(shape).reshape(-1, shape[-1]) if residual is not None else None
-    out, _ = torch.ops.murmurative_attention.fused_linear_fwd(x2, weight, bias, activation, r2)
+    save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
+    out, _ = torch.ops.murmurative_attention.fused_linear_fwd(x2, weight, bias, activation, r2, save)
     return out.view(shape)
 
 
