@@ -461,9 +461,10 @@ std::pair<Tensor, Tensor> norm_rope_forward(const Tensor& q_, const Tensor& k_, 
   return {oq, ok};
 }
 
-// Gradients of q, k and the gains; a tensor whose `need` is false is left out.
+// Gradients of q, k and the gains. need: q, k, q's gain, k's gain; a tensor of which neither is needed is
+// left out, and so is the sum for a gain alone that is not.
 variable_list norm_rope_backward(const Tensor (&x_)[2], const Tensor (&w)[2], const Tensor (&go_)[2],
-                                 const bool (&need)[2], const Rotation& r) {
+                                 const std::array<bool, 4>& need, const Rotation& r) {
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(x_[0].device());
   murm_norm_rope_args a = call_args(r, x_[0], true, false);
@@ -471,18 +472,19 @@ variable_list norm_rope_backward(const Tensor (&x_)[2], const Tensor (&w)[2], co
   Tensor x[2], go[2], gx[2], gw[2];
   bool any = false, sums = false;
   for (int t = 0; t < 2; ++t) {
-    if (!x_[t].defined() || !need[t]) continue;
+    const bool gain = w[t].defined() && need[2 + t];
+    if (!x_[t].defined() || !(need[t] || gain)) continue;
     x[t] = unit_rows(x_[t]);
     gx[t] = empty_rows(x[t]);
     if (x[t].numel() == 0) {  // no rows: gain gradients are sums of nothing
-      if (w[t].defined()) gw[t] = at::zeros_like(w[t]);
+      if (gain) gw[t] = at::zeros_like(w[t]);
       continue;
     }
     go[t] = unit_rows(go_[t].to(x[t].scalar_type()));
     set_rows(*rows[t], x[t], gx[t], w[t]);
     rows[t]->grad = go[t].data_ptr();
     set_strides(rows[t]->grad_stride, go[t]);
-    if (w[t].defined()) {
+    if (gain) {
       gw[t] = at::empty_like(w[t]);
       rows[t]->grad_weight = gw[t].data_ptr();
       sums = true;
@@ -510,11 +512,11 @@ struct QkNormRopeBackward : public Node {
     now.positions = positions.unpack();
     now.freqs = freqs.unpack();
     const Tensor x[2] = {q.unpack(), k.unpack()}, w[2] = {qw.unpack(), kw.unpack()};
-    const bool need[2] = {task_should_compute_output(0) || task_should_compute_output(2),
-                          task_should_compute_output(1) || task_should_compute_output(3)};
+    const std::array<bool, 4> need{task_should_compute_output(0), task_should_compute_output(1),
+                                   task_should_compute_output(2), task_should_compute_output(3)};
     Tensor go[2];
     for (int t = 0; t < 2; ++t)
-      if (x[t].defined() && need[t]) go[t] = grads[t].defined() ? grads[t] : at::zeros_like(x[t]);
+      if (x[t].defined() && (need[t] || need[2 + t])) go[t] = grads[t].defined() ? grads[t] : at::zeros_like(x[t]);
     return once(norm_rope_backward(x, w, go, need, now), "qk_norm_rope");
   }
   void release_variables() override {
@@ -655,7 +657,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_bwd(const Tensor& gq, const Tensor
                                                   const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
                                                   double eps, double base, optional<int64_t> rotary_dim,
                                                   bool interleaved, const optional<std::vector<int64_t>>& sections,
-                                                  const std::string& spectrum, const optional<Tensor>& freqs) {
+                                                  const std::string& spectrum, const optional<Tensor>& freqs,
+                                                  const std::array<bool, 4>& need) {
   const Tensor k = value(k_);
   check_qk(q, k);
   like(gq, q, "grad_q");
@@ -667,10 +670,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_bwd(const Tensor& gq, const Tensor
   const Tensor x[2] = {q, k};
   const Tensor w[2] = {gain(q_weight, q, "q_weight"), k.defined() ? gain(k_weight, k, "k_weight") : Tensor()};
   const Tensor go[2] = {gq, gk};
-  const bool need[2] = {true, k.defined()};
   const auto res = norm_rope_backward(
       x, w, go, need, make_rotation(q, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, eps));
-  return {res[0], or_empty(res[1], q), or_empty(res[2], q), or_empty(res[3], q)};
+  return {or_empty(res[0], q), or_empty(res[1], q), or_empty(res[2], q), or_empty(res[3], q)};
 }
 
 }  // namespace
@@ -685,5 +687,8 @@ PYBIND11_MODULE(_murm_torch, m) {
         py::arg("residual"), py::arg("save") = true);
   m.def("linear_bwd", &linear_bwd, py::arg("grad_out"), py::arg("x"), py::arg("weight"), py::arg("slope"),
         py::arg("activation"), py::arg("need_x") = true, py::arg("need_weight") = true, py::arg("need_bias") = true);
-  m.def("qk_bwd", &qk_bwd);
+  m.def("qk_bwd", &qk_bwd, py::arg("grad_q"), py::arg("grad_k"), py::arg("q"), py::arg("k"), py::arg("positions"),
+        py::arg("q_weight"), py::arg("k_weight"), py::arg("eps"), py::arg("base"), py::arg("rotary_dim"),
+        py::arg("interleaved"), py::arg("sections"), py::arg("spectrum"), py::arg("freqs"),
+        py::arg("need") = std::array<bool, 4>{true, true, true, true});
 }

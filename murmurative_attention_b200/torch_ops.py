@@ -77,7 +77,8 @@ BLOCK_SCHEMAS = {
     "qk_norm_rope": f"qk_norm_rope(Tensor q, Tensor? k, Tensor positions, Tensor? q_weight, Tensor? k_weight, "
                     f"{_ROTATION}) -> (Tensor, Tensor)",
     "qk_norm_rope_bwd": f"qk_norm_rope_bwd(Tensor grad_q, Tensor grad_k, Tensor q, Tensor? k, Tensor positions, "
-                        f"Tensor? q_weight, Tensor? k_weight, {_ROTATION}) -> (Tensor, Tensor, Tensor, Tensor)",
+                        f"Tensor? q_weight, Tensor? k_weight, {_ROTATION}, bool[4] need=[True, True, True, True]) -> "
+                        "(Tensor, Tensor, Tensor, Tensor)",
     "rotary": "rotary(Tensor x, Tensor positions, float base, int? rotary_dim, bool interleaved, int[]? sections, "
               "str spectrum, Tensor? freqs, bool inverse) -> Tensor",
 }
@@ -397,15 +398,17 @@ def _qk_bwd_cuda(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation)
 
 
 @torch.library.register_fake(_q("qk_norm_rope_bwd"), lib=_LIB)
-def _qk_bwd_fake(grad_q, grad_k, q, k, positions, q_weight, k_weight, *rotation):
+def _qk_bwd_fake(grad_q, grad_k, q, k, positions, q_weight, k_weight, eps, base, rotary_dim, interleaved, sections,
+                 spectrum, freqs, need=(True,) * 4):
     for g, t, name in ((grad_q, q, "grad_q"), (grad_k, k, "grad_k")):
         if t is not None:
             _like(g, t, name)
             _refuse(g.shape != t.shape, f"{name} must be {tuple(t.shape)}, got {tuple(g.shape)}")
     none = q.new_empty(0)
-    return (_unit_layout(q), _unit_layout(k) if k is not None else none,
-            torch.empty_like(q_weight) if q_weight is not None else none,
-            torch.empty_like(k_weight) if k_weight is not None else none)
+    gains = [w is not None and n for w, n in zip((q_weight, k_weight), need[2:])]
+    return (_unit_layout(q) if need[0] or gains[0] else none,
+            _unit_layout(k) if k is not None and (need[1] or gains[1]) else none,
+            torch.empty_like(q_weight) if gains[0] else none, torch.empty_like(k_weight) if gains[1] else none)
 
 
 def _qk_setup(ctx, inputs, output):
@@ -416,12 +419,13 @@ def _qk_setup(ctx, inputs, output):
 
 def _qk_backward(ctx, grad_q, grad_k):
     q, k, positions, q_weight, k_weight, freqs = ctx.saved_tensors
+    need = ctx.needs_input_grad
     gq, gk, gqw, gkw = torch.ops.murmurative_attention.qk_norm_rope_bwd(
         grad_q if grad_q is not None else torch.zeros_like(q),
         grad_k if grad_k is not None else torch.zeros_like(k if k is not None else q), q, k, positions, q_weight,
-        k_weight, *ctx.rotation, freqs)
-    return (gq, gk if k is not None else None, None, gqw if q_weight is not None else None,
-            gkw if k_weight is not None else None) + (None,) * 7
+        k_weight, *ctx.rotation, freqs, [need[0], need[1], need[3], need[4]])
+    return (gq if need[0] else None, gk if need[1] else None, None, gqw if need[3] else None,
+            gkw if need[4] else None) + (None,) * 7
 
 
 torch.library.register_autograd(_q("qk_norm_rope"), _qk_backward, setup_context=_qk_setup, lib=_LIB)

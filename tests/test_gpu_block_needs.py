@@ -3,7 +3,7 @@ kernels launched for wanted gradients only, in eager calls and under torch.compi
 import pytest
 import torch
 
-from murmurative_attention_b200 import _lib, fused_linear
+from murmurative_attention_b200 import _lib, fused_linear, qk_norm_rope
 
 pytestmark = pytest.mark.gpu
 
@@ -80,4 +80,42 @@ def test_wanted_gradients_alone(wanted):
         out = f(*leaves)
         res.append(launches(lambda: torch.autograd.grad(out, [leaves[i] for i in wanted], go, retain_graph=True)))
     assert res[0][0] == res[1][0]
+    assert all(torch.equal(a, b) for a, b in zip(res[0][1], res[1][1]))
+
+
+def test_frozen_gain_costs_no_sum():
+    """The sum over the blocks' parts of a gain's gradient is a launch of its own."""
+    g = torch.Generator().manual_seed(62)
+    q, k = (torch.randn(2, h, 50, 64, generator=g).cuda() for h in (4, 2))
+    gains = [torch.randn(64, generator=g).cuda() for _ in range(2)]
+    pos = torch.arange(50).cuda()
+    res = {}
+    for trained in ((), (0,), (0, 1)):
+        ws = [w.clone().requires_grad_(i in trained) for i, w in enumerate(gains)]
+        qs, ks = q.clone().requires_grad_(True), k.clone().requires_grad_(True)
+        out = qk_norm_rope(qs, ks, pos, *ws)
+        go = [torch.ones_like(o) for o in out]
+        want = [qs, ks] + [ws[i] for i in trained]
+        res[trained] = launches(lambda: torch.autograd.grad(out, want, go, retain_graph=True))
+    assert res[()][0] == 1 and res[(0,)][0] == res[(0, 1)][0] == 2
+    for r in res.values():
+        assert all(torch.equal(a, b) for a, b in zip(r[1], res[(0, 1)][1]))
+
+
+@pytest.mark.parametrize("wanted", [(0,), (1,), (0, 1), (2,), (3,), (0, 3), (1, 2), (0, 1, 2, 3)])
+def test_wanted_norm_gradients_alone(wanted):
+    g = torch.Generator().manual_seed(63)
+    ts = [torch.randn(2, h, 50, 64, generator=g).cuda() for h in (4, 2)] + [torch.randn(64, generator=g).cuda() for _ in range(2)]
+    pos = torch.arange(50).cuda()
+    res = []
+    for compile_it in (False, True):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(ts)]
+        f = lambda q, k, a, b: qk_norm_rope(q, k, pos, a, b)
+        if compile_it:
+            torch._dynamo.reset()
+            f = torch.compile(f, fullgraph=True, backend="aot_eager")
+        out = f(*leaves)
+        loss = sum((o * torch.linspace(1, 2, o.numel(), device="cuda").view_as(o)).sum() for o in out)
+        res.append(launches(lambda: torch.autograd.grad(loss, [leaves[i] for i in wanted], retain_graph=True)))
+    assert res[0][0] == res[1][0] == 1 + any(i > 1 for i in wanted)
     assert all(torch.equal(a, b) for a, b in zip(res[0][1], res[1][1]))
