@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from . import _lib
 
 _FUNCTIONS = ("murm_linear_fwd", "murm_linear_bwd", "murm_linear_workspace", "murm_linear_bwd_workspace",
@@ -16,11 +18,17 @@ _FUNCTIONS = ("murm_linear_fwd", "murm_linear_bwd", "murm_linear_workspace", "mu
 _binding = None
 
 
+def traced() -> bool:
+    """Whether this call is being traced (torch.compile, torch.export) or a dispatch mode watches it (make_fx,
+    fake tensors, counters of operations): then it has to be a registered operator, since the binding runs
+    below the dispatcher and a mode would see nothing of it but the allocation of its results."""
+    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+
+
 def binding():
     global _binding
     if _binding is None:
         lib = _lib.load_library()
-        import torch  # noqa: F401  (the binding links against it)
         try:
             from . import _murm_torch
         except ImportError as e:

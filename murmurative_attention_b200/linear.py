@@ -32,7 +32,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     Other dtypes raise TypeError, an unknown activation ValueError, CPU tensors and shapes that do not
     fit RuntimeError.
     """
-    if torch.compiler.is_compiling():
+    if _native.traced():
         from .torch_ops import fused_linear as registered
         return registered(x, weight, bias, activation, residual)
     return _native.binding().fused_linear(x, weight, bias, activation, residual)

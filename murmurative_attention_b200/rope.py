@@ -39,7 +39,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     Other dtypes raise TypeError, an unknown spectrum ValueError, CPU tensors and shapes that do not
     fit RuntimeError.
     """
-    if torch.compiler.is_compiling():
+    if _native.traced():
         oq, ok = torch.ops.murmurative_attention.qk_norm_rope(q, k, positions, q_weight, k_weight, eps, base, rotary_dim,
                                                               interleaved, sections, spectrum, freqs)
         return oq, ok if k is not None else None
@@ -66,7 +66,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, *, base: float = 10000.0, r
 
     Returns a tensor in x's layout. Differentiable with respect to x (the inverse rotation).
     """
-    if torch.compiler.is_compiling():
+    if _native.traced():
         return torch.ops.murmurative_attention.rotary(x, positions, base, rotary_dim, interleaved, sections, spectrum,
                                                       freqs, inverse)
     return _native.binding().rotary(x, positions, base, rotary_dim, interleaved, sections, spectrum, freqs, inverse)

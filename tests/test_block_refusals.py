@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from murmurative_attention_b200 import _lib, _native, torch_ops
+from murmurative_attention_b200 import _lib, _native, fused_linear, qk_norm_rope, rotary, torch_ops
 
 NS = torch.ops.murmurative_attention
 
@@ -130,3 +130,16 @@ def test_bias_gradient_needs_no_more_than_its_chunks(rows, n, act):
     need = ctypes.c_size_t(0)
     assert _lib.load_library().murm_linear_bwd_workspace(ctypes.byref(a), ctypes.byref(need)) == 0
     assert need.value <= (rows // 24 + 1) * n * 4 * (rows > 16) + 256
+
+
+def test_public_functions_take_fake_tensors(fake):
+    """Under a fake mode the functions give fakes of their results, and refuse what does not fit."""
+    x, w = fake(2, 3, 64), fake(32, 64)
+    assert fused_linear(x, w, fake(32), activation="silu").shape == (2, 3, 32)
+    with pytest.raises(RuntimeError):
+        fused_linear(x, fake(32, 65))
+    q = fake(2, 5, 4, 64).transpose(1, 2)
+    pos = fake(5, dtype=torch.int64)
+    assert rotary(q, pos).stride() == q.stride()
+    oq, ok = qk_norm_rope(q, q[:, :2], pos)
+    assert oq.shape == q.shape and ok.shape == (2, 2, 5, 64)

@@ -42,3 +42,30 @@ def test_jit_trace_raises(name):
     f, inputs = calls()[name]
     with pytest.raises(RuntimeError, match="torch.jit.trace"):
         torch.jit.trace(f, tuple(inputs), check_trace=False)
+
+
+@pytest.mark.parametrize("name", ["linear", "qk", "rotary"])
+def test_dispatch_modes_see_the_operators(name):
+    """make_fx's graph gives the call's results on other inputs; a mode that records calls finds the operator."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    f, inputs = calls()[name]
+    graph = make_fx(f)(*inputs)
+    others = [t + 0.25 for t in inputs]
+    torch.testing.assert_close(graph(*others), f(*others))
+    seen = []
+    with Record():
+        out = f(*inputs)
+    assert any("murmurative_attention" in s for s in seen) and torch.equal(out, f(*inputs))
+    leaves = [t.clone().requires_grad_(True) for t in inputs]
+    want = torch.autograd.grad(f(*leaves).square().sum(), leaves, allow_unused=True)
+    with Record():
+        loss = f(*leaves).square().sum()
+    for a, b in zip(torch.autograd.grad(loss, leaves, allow_unused=True), want):
+        assert (a is None or not bool(a.any())) if b is None else torch.equal(a, b)
