@@ -14,8 +14,9 @@
 // residual -> 64-byte swizzled rows in shared memory -> TMA store (or plain stores where the
 // result's rows are not 16-byte aligned).
 //
-// fp32 operands are three bf16 planes; the products of planes (i, j) with i + j <= 2 carry them to
-// 2^-24, added smallest first into the same fp32 accumulator. Products with few tiles and a long K split
+// fp32 operands are three bf16 planes, the terms cut and not rounded; the products of planes (i, j) with
+// i + j <= 2 are added smallest first into the same fp32 accumulator. The pairs left out, (1,2) and (2,1)
+// before all, are up to 2^-21 of a product and 2^-24.7 on average, always with its sign. Products with few tiles and a long K split
 // K; the parts' fp32 sums go to the workspace and k_split_sum adds them in order and runs the epilogue. So
 // do fp32 products of a long K, whose items change accumulators on the way (kSegment).
 #include <cudaTypedefs.h>

@@ -60,8 +60,8 @@ __device__ __forceinline__ void store_operand(const Operand& o, int64_t at, cons
 // columns, up to the block), the others on further rows; a chunk of rows. db sums dz unrounded, in
 // fp32: a thread's rows in order, then the block's row groups in order, then (k_col_sum, if there are several) the chunks.
 //
-// Bound by memory: dy and the slopes read once, dz written once; 32768 x 4096 bf16 takes 129 us
-// (6.3 TB/s). A row's columns go to neighbouring threads and a thread issues kDzDepth rows' loads
+// Bound by memory: dy and the slopes read once, dz written once; 32768 x 4096 bf16 takes 135 us
+// (6.0 TB/s; 127 with slopes in equal steps alone). A row's columns go to neighbouring threads and a thread issues kDzDepth rows' loads
 // together; with a bounds check at each of them they went out one by one (180 us), so full batches
 // run without and single rows follow.
 constexpr int kDzDepth = 4;
@@ -169,9 +169,9 @@ DzShape dz_shape(const murm_linear_bwd_args& a) {
   s.blocks_x = (int)(((int64_t)N + s.cols * s.v - 1) / (s.cols * s.v));
   // Two rounds of three blocks per SM, so that the last ones leave little idle. With slopes one round
   // where two would leave a thread less than 64 rows, and 24 rows per chunk at least (bf16 8192 x 4096,
-  // gradients of 64 inputs with it: one round of 37 rows 70 us, 32 rows in 1.15 rounds 78; 4096 x 1024:
-  // chunks of 24 rows 18.2, of 32 19.1, of 48 20.6). Without them, half the bytes, 32 rows and two rounds
-  // (8192 x 4096: 42.0, one round 43.5).
+  // gradients of 64 inputs with it: one round of 37 rows 71 us, 32 rows in 1.15 rounds 8 more; 4096 x 1024:
+  // chunks of 24 rows 19.0, of 32 and 48 0.9 and 2.4 more). Without them, half the bytes, 32 rows and two rounds
+  // (8192 x 4096: 41.2, one round 1.5 more).
   const bool slopes = a.activation != MURM_ACT_NONE;
   const int wave = 148 * 3 / s.blocks_x, least = slopes ? 24 : 32;
   int most = 2 * wave;
