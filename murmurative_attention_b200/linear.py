@@ -29,8 +29,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     reads x, weight and the activation's slopes, which the forward saves in two bytes per element of
     16-bit outputs and four of fp32 ones (none without an activation).
 
-    Other dtypes raise TypeError, an unknown activation ValueError, CPU tensors and shapes that do not
-    fit RuntimeError.
+    Other dtypes raise TypeError, an unknown activation ValueError, CPU tensors, shapes that do not fit and
+    torch.jit.trace RuntimeError, forward-mode differentiation NotImplementedError. torch.compile, make_fx and
+    other dispatch modes see a registered operator.
     """
     if _native.traced():
         from .torch_ops import fused_linear as registered

@@ -36,8 +36,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     Returns (q, k) normed and rotated, in the inputs' layouts (k None when it was None).
     Differentiable (once) with respect to q, k and the gains.
 
-    Other dtypes raise TypeError, an unknown spectrum ValueError, CPU tensors and shapes that do not
-    fit RuntimeError.
+    Other dtypes raise TypeError, an unknown spectrum ValueError, CPU tensors, shapes that do not fit and
+    torch.jit.trace RuntimeError, forward-mode differentiation NotImplementedError. torch.compile, make_fx and
+    other dispatch modes see a registered operator.
     """
     if _native.traced():
         oq, ok = torch.ops.murmurative_attention.qk_norm_rope(q, k, positions, q_weight, k_weight, eps, base, rotary_dim,
